@@ -1,0 +1,453 @@
+// Root-mean-square norm of rows for gfx950 behind the C ABI of include/ovl_norm.h: with the residual's addition, with an
+// 8-bit output and its scales, and the gradient.
+//
+// Mathematics.  s = x + residual as stored, rstd = 1 / sqrt(mean s^2 + eps), y = s rstd w.  With t = dy w and n = s rstd
+// the gradient is ds = rstd (t - n mean(t n)) + dsummed, dw = sum over rows of dy n.
+//
+// Work layout: LANES lanes share a row (a wavefront, four or sixteen of them) and hold all of it in registers, HELD
+// vectors of eight columns per lane, so everything is read once and written once: the kernels are bound by memory.  The
+// statistics of a row are one exchange between its wavefronts.  Rows need not start on vector boundaries: the vectors are
+// accessed with the alignment of an element, a row's last, partial vector element by element.
+#include <math.h>
+#include <stdint.h>
+#include <string>
+#include <type_traits>
+
+#include "ovl_lane.h"
+#include "ovl_norm.h"
+
+#define OVL_OK 0
+#define OVL_EHIP 4
+#define OVL_EINVAL 6
+
+using ovl_lane::bf16;
+using ovl_lane::f16;
+using ovl_lane::narrow;
+using ovl_lane::widen;
+
+namespace {
+
+constexpr int VEC = 8;
+constexpr float E4M3_MAX = 448.0f;
+
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) pack { T v[VEC]; };
+
+// Eight columns from `c` on of a row, zero past its end.
+template <typename T>
+__device__ __forceinline__ void load_vec(float (&to)[VEC], const T* row, uint32_t c, uint32_t columns) {
+    if (c + VEC <= columns) {
+        const pack<T> raw = *reinterpret_cast<const pack<T>*>(row + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) to[i] = widen<T>(raw.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) to[i] = c + i < columns ? widen<T>(row[c + i]) : 0.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(const float (&x)[VEC], T* row, uint32_t c, uint32_t columns) {
+    if (c + VEC <= columns) {
+        pack<T> out;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out.v[i] = narrow<T>(x[i]);
+        *reinterpret_cast<pack<T>*>(row + c) = out;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (c + i < columns) row[c + i] = narrow<T>(x[i]);
+    }
+}
+
+// The weights are float32 or of the rows' type.
+template <typename T>
+__device__ __forceinline__ void load_weights(float (&to)[VEC], const void* weight, bool wide, uint32_t c, uint32_t columns) {
+    if (wide) load_vec<float>(to, static_cast<const float*>(weight), c, columns);
+    else load_vec<T>(to, static_cast<const T*>(weight), c, columns);
+}
+
+struct add_op { __device__ static __forceinline__ float of(float a, float b) { return a + b; } };
+struct max_op { __device__ static __forceinline__ float of(float a, float b) { return fmaxf(a, b); } };
+
+// Over the sixteen lanes of a row of lanes, resp. over the wavefront; every lane receives the result.
+template <typename OP> __device__ __forceinline__ float row_all(float x) {
+    x = OP::of(x, ovl_lane::row_round<8>(x));
+    x = OP::of(x, ovl_lane::row_round<4>(x));
+    x = OP::of(x, ovl_lane::row_round<2>(x));
+    return OP::of(x, ovl_lane::row_round<1>(x));
+}
+template <typename OP> __device__ __forceinline__ float wave_all(float x) {
+    x = row_all<OP>(x);
+    float a = x, b = x;
+    ovl_lane::swap_rows(a, b);
+    x = OP::of(a, b);
+    a = x;
+    b = x;
+    ovl_lane::swap_halves(a, b);
+    return OP::of(a, b);
+}
+
+// Two results over all lanes of a row of the matrix: a sum, and a second value by OP.  `lds` is not read again before
+// the next barrier after this call, so two calls need a barrier, or two places, between them.
+template <int LANES, typename OP>
+__device__ __forceinline__ void across(float& sum, float& other, float (*lds)[2]) {
+    sum = wave_all<add_op>(sum);
+    other = wave_all<OP>(other);
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        const uint32_t wave = threadIdx.x / 64u;
+        if ((threadIdx.x & 63u) == 0u) { lds[wave][0] = sum; lds[wave][1] = other; }
+        __syncthreads();
+        sum = lds[0][0];
+        other = lds[0][1];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) { sum += lds[i][0]; other = OP::of(other, lds[i][1]); }
+    }
+}
+
+struct norm_args {
+    uint32_t rows, columns;
+    float eps, over_columns;
+    const void *x, *residual, *weight;
+    int64_t x_stride, residual_stride;
+    int32_t wide_weight;
+};
+
+// R: the type of the residual and of s.  QUANTIZED: q and scales instead of y; GROUPED: a scale for each 128 columns
+// (which are the 16 lanes of one row of lanes), else one for the row.
+template <typename T, typename R, int LANES, int HELD, bool QUANTIZED, bool GROUPED>
+__global__ void __launch_bounds__(LANES > 256 ? LANES : 256)
+norm_forward_kernel(norm_args p, T* y, R* summed, uint8_t* q, float* scales) {
+    constexpr uint32_t PER = LANES > 256 ? 1 : 256 / LANES;     // rows of a workgroup
+    __shared__ float lds[LANES / 64][2];
+    const uint32_t lane = threadIdx.x % LANES;
+    const uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / LANES;
+    if (row >= p.rows) return;              // with more than one row per workgroup there is no barrier
+    const T* x = static_cast<const T*>(p.x) + (int64_t)row * p.x_stride;
+    float s[HELD][VEC];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) load_vec<T>(s[h], x, (h * LANES + lane) * VEC, p.columns);
+    if (p.residual != nullptr) {
+        const R* residual = static_cast<const R*>(p.residual) + (int64_t)row * p.residual_stride;
+        R* to = summed + row * p.columns;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const uint32_t c = (h * LANES + lane) * VEC;
+            float more[VEC];
+            load_vec<R>(more, residual, c, p.columns);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s[h][i] = widen<R>(narrow<R>(s[h][i] + more[i]));
+            store_vec<R>(s[h], to, c, p.columns);
+        }
+    }
+    float squares = 0.0f, largest = 0.0f;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) squares = fmaf(s[h][i], s[h][i], squares);
+    float w[HELD][VEC];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
+        if (QUANTIZED && !GROUPED)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) largest = fmaxf(largest, fabsf(s[h][i] * w[h][i]));
+    }
+    across<LANES, max_op>(squares, largest, lds);
+    const float rstd = ovl_lane::rsq_(fmaf(squares, p.over_columns, p.eps));
+    // one scale for the row: max |y| = rstd max |s w|
+    const float row_largest = largest * rstd;
+    if (QUANTIZED && !GROUPED && lane == 0u) scales[row] = row_largest > 0.0f ? row_largest / E4M3_MAX : 1.0f;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const uint32_t c = (h * LANES + lane) * VEC;
+        float out[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) out[i] = s[h][i] * rstd * w[h][i];
+        if constexpr (!QUANTIZED) {
+            store_vec<T>(out, y + row * p.columns, c, p.columns);
+        } else {
+            float top = row_largest;
+            if constexpr (GROUPED) {
+                top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(out[i]));
+                top = row_all<max_op>(top);
+                const uint32_t group = c / 128u, groups = (p.columns + 127u) / 128u;
+                if ((lane & 15u) == 0u && group < groups)
+                    scales[row * groups + group] = top > 0.0f ? top / E4M3_MAX : 1.0f;
+            }
+            const float inverse = top > 0.0f ? E4M3_MAX / top : 0.0f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) out[i] *= inverse;
+            struct __attribute__((packed, aligned(1))) bytes { uint32_t v[2]; } packed;
+            packed.v[0] = ovl_lane::e4m3x4(out[0], out[1], out[2], out[3]);
+            packed.v[1] = ovl_lane::e4m3x4(out[4], out[5], out[6], out[7]);
+            uint8_t* to = q + row * p.columns + c;
+            if (c + VEC <= p.columns) *reinterpret_cast<bytes*>(to) = packed;
+            else
+#pragma unroll
+                for (uint32_t i = 0; i < VEC; ++i)
+                    if (c + i < p.columns) to[i] = (uint8_t)(packed.v[i / 4u] >> (8u * (i % 4u)));
+        }
+    }
+}
+
+struct norm_gradient_args {
+    const void *d_y, *d_summed;
+    int64_t d_y_stride, d_summed_stride;
+    void *d_x, *d_residual;
+    float* part;                            // [rows of parts][columns]
+};
+
+// A team of LANES lanes takes rows `team`, team + teams, ... and keeps its sums for the weights in registers.
+template <typename T, typename R, int LANES, int HELD>
+__global__ void __launch_bounds__(LANES > 256 ? LANES : 256)
+norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
+    constexpr uint32_t PER = LANES > 256 ? 1 : 256 / LANES;
+    __shared__ float lds[2][LANES / 64][2];
+    const uint32_t lane = threadIdx.x % LANES;
+    const uint32_t team = blockIdx.x * PER + threadIdx.x / LANES;
+    if (team >= teams) return;              // with more than one team per workgroup there is no barrier
+    float dw[HELD][VEC];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) dw[h][i] = 0.0f;
+    uint32_t turn = 0;
+    for (uint64_t row = team; row < p.rows; row += teams, turn ^= 1u) {
+        const R* x = static_cast<const R*>(p.x) + (int64_t)row * p.x_stride;
+        const T* d_y = static_cast<const T*>(g.d_y) + (int64_t)row * g.d_y_stride;
+        float n[HELD][VEC], t[HELD][VEC];
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const uint32_t c = (h * LANES + lane) * VEC;
+            load_vec<R>(n[h], x, c, p.columns);
+            load_vec<T>(t[h], d_y, c, p.columns);
+        }
+        // one exchange for both: rstd comes from the sum of s^2, and mean(t n) = rstd mean(t s)
+        float squares = 0.0f, dot = 0.0f, w[HELD][VEC];
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                squares = fmaf(n[h][i], n[h][i], squares);
+                dot = fmaf(t[h][i] * w[h][i], n[h][i], dot);
+            }
+        }
+        across<LANES, add_op>(squares, dot, lds[turn]);
+        const float rstd = ovl_lane::rsq_(fmaf(squares, p.over_columns, p.eps));
+        const float mean = dot * rstd * p.over_columns;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const uint32_t c = (h * LANES + lane) * VEC;
+            float out[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float unit = n[h][i] * rstd;
+                dw[h][i] = fmaf(t[h][i], unit, dw[h][i]);
+                out[i] = rstd * fmaf(-mean, unit, t[h][i] * w[h][i]);
+            }
+            if (g.d_summed != nullptr) {
+                float more[VEC];
+                load_vec<R>(more, static_cast<const R*>(g.d_summed) + (int64_t)row * g.d_summed_stride, c, p.columns);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) out[i] += more[i];
+            }
+            if (g.d_x != nullptr) store_vec<T>(out, static_cast<T*>(g.d_x) + row * p.columns, c, p.columns);
+            if (g.d_residual != nullptr) store_vec<R>(out, static_cast<R*>(g.d_residual) + row * p.columns, c, p.columns);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        store_vec<float>(dw[h], g.part + (uint64_t)team * p.columns, (h * LANES + lane) * VEC, p.columns);
+}
+
+// Adds the teams' parts up: 64 columns per workgroup, four wavefronts share the parts, in a fixed order.
+template <typename W>
+__global__ void __launch_bounds__(256)
+norm_sum_kernel(const float* part, uint32_t columns, uint32_t teams, W* d_weight) {
+    __shared__ float lds[4][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, c = blockIdx.x * 64u + lane;
+    float sum = 0.0f;
+    if (c < columns)
+#pragma unroll 8
+        for (uint32_t k = wave; k < teams; k += 4u) sum += part[(uint64_t)k * columns + c];
+    lds[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0u && c < columns) d_weight[c] = narrow<W>((lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]));
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------------
+
+thread_local std::string g_last_error;
+
+int fail(const std::string& detail) {
+    g_last_error = detail;
+    return OVL_EINVAL;
+}
+
+int after_launch(const char* who) {
+    const hipError_t err = hipPeekAtLastError();
+    if (err != hipSuccess) {
+        (void)hipGetLastError();
+        g_last_error = std::string(who) + ": " + hipGetErrorString(err);
+        return OVL_EHIP;
+    }
+    return OVL_OK;
+}
+
+bool known(int32_t dtype) { return dtype == OVL_NORM_FLOAT16 || dtype == OVL_NORM_FLOAT32 || dtype == OVL_NORM_BFLOAT16; }
+
+int check(const char* who, const ovl_norm* p) {
+    const std::string name(who);
+    if (p == nullptr) return fail(name + ": null norm");
+    if (p->rows == 0 || p->columns == 0) return fail(name + ": sizes must be positive");
+    if (p->columns > 32768u) return fail(name + ": at most 32768 columns");
+    if (p->rows > (1u << 31) - 1u) return fail(name + ": too many rows for one launch");
+    if (!known(p->dtype)) return fail(name + ": unknown element type");
+    if (p->residual_dtype != p->dtype && p->residual_dtype != OVL_NORM_FLOAT32) return fail(name + ": the residual must be of the rows' type or float32");
+    if (p->weight_dtype != p->dtype && p->weight_dtype != OVL_NORM_FLOAT32) return fail(name + ": the weight must be of the rows' type or float32");
+    if (p->x == nullptr || p->weight == nullptr) return fail(name + ": null tensor");
+    return OVL_OK;
+}
+
+norm_args make_args(const ovl_norm* p) {
+    return norm_args{p->rows, p->columns, p->eps, 1.0f / (float)p->columns, p->x, p->residual, p->weight, p->x_stride,
+                     p->residual_stride, p->weight_dtype == OVL_NORM_FLOAT32 ? 1 : 0};
+}
+
+// Lanes per row and vectors per lane: a wavefront up to 2048 columns, four up to 8192, sixteen up to 32768, at most four
+// vectors of eight columns per lane.
+template <typename F> void by_columns(uint32_t columns, F&& call) {
+    const uint32_t vectors = (columns + VEC - 1) / VEC;
+#define OVL_NORM_HELD(LANES)                                                                                                   \
+    {                                                                                                                         \
+        const uint32_t held = (vectors + LANES - 1) / LANES;                                                                  \
+        if (held <= 1) call(std::integral_constant<int, LANES>(), std::integral_constant<int, 1>());                          \
+        else if (held <= 2) call(std::integral_constant<int, LANES>(), std::integral_constant<int, 2>());                     \
+        else call(std::integral_constant<int, LANES>(), std::integral_constant<int, 4>());                                    \
+    }
+    if (vectors <= 4 * 64) OVL_NORM_HELD(64)
+    else if (vectors <= 4 * 256) OVL_NORM_HELD(256)
+    else OVL_NORM_HELD(1024)
+#undef OVL_NORM_HELD
+}
+
+template <typename F> void by_types(const ovl_norm* p, F&& call) {
+    const bool wide = p->residual_dtype == OVL_NORM_FLOAT32;
+    switch (p->dtype) {
+        case OVL_NORM_FLOAT32: call(float(), float()); break;
+        case OVL_NORM_FLOAT16: if (wide) call(f16(), float()); else call(f16(), f16()); break;
+        default: if (wide) call(bf16(), float()); else call(bf16(), bf16()); break;
+    }
+}
+
+template <int LANES> constexpr uint32_t threads_of() { return LANES > 256 ? LANES : 256; }
+
+// Teams of the backward pass: as many as fill the compute units twice; a team's part of the weight gradient is written
+// and read once, so few rows get few teams.
+uint32_t teams_for(const ovl_norm* p) {
+    const uint32_t most = p->columns <= 2048u ? 4096u : p->columns <= 8192u ? 1024u : 512u;
+    const uint32_t few = (p->rows + 3u) / 4u;
+    return few < most ? few : most;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* ovl_norm_last_error(void) { return g_last_error.c_str(); }
+
+int ovl_norm_forward(const ovl_norm* p, void* y, void* summed, void* hip_stream) {
+    const int rc = check("ovl_norm_forward", p);
+    if (rc != OVL_OK) return rc;
+    if (y == nullptr || (p->residual != nullptr && summed == nullptr)) return fail("ovl_norm_forward: null tensor");
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    const norm_args args = make_args(p);
+    by_types(p, [&](auto t, auto r) {
+        typedef decltype(t) T;
+        typedef decltype(r) R;
+        by_columns(p->columns, [&](auto lanes, auto held) {
+            constexpr int LANES = decltype(lanes)::value, HELD = decltype(held)::value;
+            constexpr uint32_t THREADS = threads_of<LANES>(), PER = THREADS / LANES;
+            hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, false, false>), dim3((p->rows + PER - 1) / PER),
+                               dim3(THREADS), 0, stream, args, static_cast<T*>(y), static_cast<R*>(summed),
+                               static_cast<uint8_t*>(nullptr), static_cast<float*>(nullptr));
+        });
+    });
+    return after_launch("ovl_norm_forward");
+}
+
+int ovl_norm_forward_quantized(const ovl_norm* p, uint32_t group_columns, void* q, float* scales, void* summed,
+                               void* hip_stream) {
+    const int rc = check("ovl_norm_forward_quantized", p);
+    if (rc != OVL_OK) return rc;
+    if (group_columns != 0u && group_columns != 128u)
+        return fail("ovl_norm_forward_quantized: a scale spans the row or 128 columns");
+    if (q == nullptr || scales == nullptr || (p->residual != nullptr && summed == nullptr))
+        return fail("ovl_norm_forward_quantized: null tensor");
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    const norm_args args = make_args(p);
+    by_types(p, [&](auto t, auto r) {
+        typedef decltype(t) T;
+        typedef decltype(r) R;
+        by_columns(p->columns, [&](auto lanes, auto held) {
+            constexpr int LANES = decltype(lanes)::value, HELD = decltype(held)::value;
+            constexpr uint32_t THREADS = threads_of<LANES>(), PER = THREADS / LANES;
+            const dim3 grid((p->rows + PER - 1) / PER);
+            if (group_columns != 0u)
+                hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, true, true>), grid, dim3(THREADS), 0, stream, args,
+                                   static_cast<T*>(nullptr), static_cast<R*>(summed),
+                                   static_cast<uint8_t*>(q), scales);
+            else
+                hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, true, false>), grid, dim3(THREADS), 0, stream, args,
+                                   static_cast<T*>(nullptr), static_cast<R*>(summed),
+                                   static_cast<uint8_t*>(q), scales);
+        });
+    });
+    return after_launch("ovl_norm_forward_quantized");
+}
+
+uint64_t ovl_norm_workspace_bytes(const ovl_norm* p) {
+    if (check("ovl_norm_workspace_bytes", p) != OVL_OK) return 0;
+    return (uint64_t)teams_for(p) * p->columns * sizeof(float);
+}
+
+int ovl_norm_backward(const ovl_norm* p, const void* d_y, int64_t d_y_stride, const void* d_summed,
+                      int64_t d_summed_stride, void* d_x, void* d_residual, void* d_weight, void* workspace,
+                      uint64_t workspace_bytes, void* hip_stream) {
+    const int rc = check("ovl_norm_backward", p);
+    if (rc != OVL_OK) return rc;
+    if (d_y == nullptr || d_weight == nullptr) return fail("ovl_norm_backward: null tensor");
+    const uint32_t teams = teams_for(p);
+    if (workspace == nullptr || workspace_bytes < (uint64_t)teams * p->columns * sizeof(float) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0)
+        return fail("ovl_norm_backward: workspace too small or not 4-byte aligned");
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    const norm_args args = make_args(p);
+    norm_gradient_args g{d_y, d_summed, d_y_stride, d_summed_stride, d_x, d_residual, static_cast<float*>(workspace)};
+    by_types(p, [&](auto t, auto r) {
+        typedef decltype(t) T;
+        typedef decltype(r) R;
+        by_columns(p->columns, [&](auto lanes, auto held) {
+            constexpr int LANES = decltype(lanes)::value, HELD = decltype(held)::value;
+            constexpr uint32_t THREADS = threads_of<LANES>(), PER = THREADS / LANES;
+            hipLaunchKernelGGL((norm_backward_kernel<T, R, LANES, HELD>), dim3((teams + PER - 1) / PER), dim3(THREADS), 0,
+                               stream, args, g, teams);
+        });
+        const dim3 grid((p->columns + 63u) / 64u);
+        if (p->weight_dtype == OVL_NORM_FLOAT32)
+            hipLaunchKernelGGL((norm_sum_kernel<float>), grid, dim3(256), 0, stream, static_cast<const float*>(workspace),
+                               p->columns, teams, static_cast<float*>(d_weight));
+        else
+            hipLaunchKernelGGL((norm_sum_kernel<T>), grid, dim3(256), 0, stream, static_cast<const float*>(workspace),
+                               p->columns, teams, static_cast<T*>(d_weight));
+    });
+    return after_launch("ovl_norm_backward");
+}
+
+}  // extern "C"

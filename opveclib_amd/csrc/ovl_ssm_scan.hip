@@ -1,0 +1,1011 @@
+// Selective state space scan for gfx950 behind the C ABI of include/ovl_ssm.h: forward, backward, one-token step.
+//
+// Mathematics.  Every (sequence, channel, state entry) is a linear recurrence of its own, h[t] = a[t] h[t-1] + b[t] with
+// a[t] = exp(dt[t] A) and b[t] = dt[t] u[t] B[t]; the output sums over the state entries, y[t] = sum C[t] h[t].  The
+// gradient is the same recurrence from the other end: g[t] = C[t] dy[t] + r[t+1], r[t] = a[t] g[t].
+//
+// Work layout.  A quad of lanes owns one channel, each of its lanes S of the channel's (up to 64) state entries in
+// registers; a wavefront owns 16 channels, a workgroup of four wavefronts 64 neighbouring channels of one group and walks
+// along the tokens in tiles of 16.  What depends on (token, channel) only - the loads, softplus, the gate - is done once
+// for four tokens in the four lanes of the quad and handed round with lane moves that are part of the consuming
+// instruction; the sums over the state entries end in an exchange inside the quad that leaves every lane with its own
+// token.  B and C, which all channels of the workgroup share, go through LDS as float32, one barrier per tile, the next
+// tile's loads in flight.
+//
+// Bound.  Per state entry and token: one multiplication and one exponential (two issue slots) for the decay, one
+// multiplication and two fused multiply-adds: 24 clocks of a SIMD per wavefront, measured; at 16 state entries that is
+// more than what the loads and stores take, so the vector ALU bounds the scan.
+//
+// Splitting the length.  A sequence is sequential; few channels leave compute units idle.  Then the tokens are split into
+// chunks: one pass computes every chunk's effect on a zero state (the decay of a chunk needs only the sum of its dt), a
+// small kernel joins the chunks' states, and the full pass starts every chunk from its true state.  The price is a second
+// evaluation of every decay, so the split is made only where it pays (chunks_for below).
+#include <math.h>
+
+#include "ovl_lane.h"
+#include "ovl_ssm_host.h"
+
+using ovl_lane::bf16;
+using ovl_lane::f16;
+using ovl_lane::narrow;
+using ovl_lane::widen;
+
+namespace {
+
+constexpr uint32_t TILE = 16;               // tokens per tile; states are kept for the backward pass once per tile
+constexpr uint32_t QUADS = TILE / 4;        // groups of four tokens
+constexpr uint32_t WAVES = 4;
+constexpr uint32_t THREADS = 64 * WAVES;
+constexpr uint32_t BLOCK = 16 * WAVES;      // channels of a workgroup
+
+constexpr float LOG2E = 0x1.715476p+0f, LN2 = 0x1.62e43p-1f;
+
+template <typename T> struct sequence { const T* data; int64_t batch_stride, token_stride; };
+template <typename T> struct vectors { const T* data; int64_t batch_stride, token_stride, group_stride; };
+
+template <typename T> struct scan_args {
+    uint32_t batch, length, channels, state, groups;
+    uint32_t per_group, blocks;             // channels per group, workgroups per group
+    uint32_t tiles, chunks, chunk_tiles;    // tiles of the length, chunks, tiles per chunk
+    int32_t  softplus;
+    sequence<T> u, delta, z;
+    vectors<T> B, C;
+    const float *A, *D, *delta_bias, *entering;
+    const int32_t* lengths;
+};
+
+// Where a workgroup works: sequence, group, block of channels, chunk.
+struct place {
+    uint32_t b, g, block, chunk;
+    uint32_t q, channel;                    // lane of the quad; channel (clamped to a valid one)
+    bool active;                            // whether the channel is one of the group's
+    uint32_t first, last;                   // tiles
+    uint32_t end;                           // first token behind the sequence
+};
+
+template <typename T>
+__device__ __forceinline__ place find_place(const scan_args<T>& p, uint32_t chunk_base, uint32_t chunks) {
+    place w;
+    uint32_t id = blockIdx.x;
+    w.chunk = chunk_base + id % chunks;
+    id /= chunks;
+    w.block = id % p.blocks;
+    id /= p.blocks;
+    w.g = id % p.groups;
+    w.b = id / p.groups;
+    w.q = threadIdx.x & 3u;
+    uint32_t c = w.block * BLOCK + threadIdx.x / 4u;
+    w.active = c < p.per_group;
+    c = w.active ? c : p.per_group - 1u;
+    w.channel = w.g * p.per_group + c;
+    w.first = w.chunk * p.chunk_tiles;
+    w.last = min(w.first + p.chunk_tiles, p.tiles);
+    w.end = p.length;
+    if (p.lengths != nullptr) {
+        const int32_t n = p.lengths[w.b];
+        w.end = n < 0 ? 0u : min((uint32_t)n, p.length);
+    }
+    return w;
+}
+
+// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|; what 1 + e rounds away is put back, so that the result keeps its
+// relative precision where it is small (time steps of 0.001 are ordinary).  The product |x| log2(e) is carried to twice
+// the precision for the same reason.
+__device__ __forceinline__ float softplus_(float x) {
+    const float ax = fabsf(x);
+    const float p = -ax * LOG2E;
+    const float low = fmaf(-ax, LOG2E, -p);
+    float e = ovl_lane::exp2_(p);
+    e = ax < 100.0f ? fmaf(e * LN2, low, e) : e;
+    const float w = 1.0f + e;
+    const float lost = e - (w - 1.0f);
+    const float log1p = fmaf(lost, ovl_lane::rcp_(w), ovl_lane::log2_(w) * LN2);
+    return fmaxf(x, 0.0f) + log1p;
+}
+
+__device__ __forceinline__ float sigmoid_(float x) { return ovl_lane::rcp_(1.0f + ovl_lane::exp2_(-x * LOG2E)); }
+
+// Every lane's raw elements of the four groups of tokens of a tile: token t0 + 4 j + q.  Tokens behind the length are
+// read as the last one (the values are not used).
+template <typename T>
+__device__ __forceinline__ void load_tile(T (&to)[QUADS], const sequence<T>& s, const place& w, uint32_t t0, uint32_t length) {
+    const T* base = s.data + (int64_t)w.b * s.batch_stride + w.channel;
+#pragma unroll
+    for (uint32_t j = 0; j < QUADS; ++j) to[j] = base[(int64_t)min(t0 + 4u * j + w.q, length - 1u) * s.token_stride];
+}
+
+// The elements of a tile of B or C that this thread takes to LDS, NP = 4 S entries per token.
+template <typename T, int S> struct vector_stage {
+    static constexpr uint32_t NP = 4 * S, ALL = TILE * NP, PER = (ALL + THREADS - 1) / THREADS;
+    T raw[PER];
+    __device__ __forceinline__ void load(const vectors<T>& v, const place& w, uint32_t t0, uint32_t length, uint32_t n) {
+        const T* base = v.data + (int64_t)w.b * v.batch_stride + (int64_t)w.g * v.group_stride;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint32_t at = threadIdx.x + i * THREADS;
+            raw[i] = base[(int64_t)min(t0 + at / NP, length - 1u) * v.token_stride + min(at % NP, n - 1u)];
+        }
+    }
+    // Entries past the state and tokens behind the sequence become zero: they then add nothing anywhere.
+    __device__ __forceinline__ void store(float* lds, const place& w, uint32_t t0, uint32_t n) const {
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint32_t at = threadIdx.x + i * THREADS;
+            if (at < ALL) lds[at] = (at % NP < n && t0 + at / NP < w.end) ? widen<T>(raw[i]) : 0.0f;
+        }
+    }
+};
+
+template <int S> __device__ __forceinline__ void load_states(float (&h)[S], const float* from) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) h[s] = from[s];
+}
+template <int S> __device__ __forceinline__ void store_states(const float (&h)[S], float* to) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) to[s] = h[s];
+}
+
+// S entries of a [.., state] tensor for the lane's part of the state, zero past the end.
+template <int S>
+__device__ __forceinline__ void load_entries(float (&h)[S], const float* row, uint32_t q, uint32_t n) {
+#pragma unroll
+    for (uint32_t s = 0; s < S; ++s) {
+        const uint32_t at = q * S + s;
+        h[s] = at < n ? row[at] : 0.0f;
+    }
+}
+template <int S>
+__device__ __forceinline__ void store_entries(const float (&h)[S], float* row, uint32_t q, uint32_t n) {
+#pragma unroll
+    for (uint32_t s = 0; s < S; ++s) {
+        const uint32_t at = q * S + s;
+        if (at < n) row[at] = h[s];
+    }
+}
+
+__device__ __forceinline__ float quad_sum(float x) {
+    x += ovl_lane::quad_xor1(x);
+    return x + ovl_lane::quad_xor2(x);
+}
+
+// Four values per lane, one for each token of the quad: lane q receives the sum over the quad of value q.
+__device__ __forceinline__ float quad_scatter_sum(const float (&v)[4], uint32_t q) {
+    const bool odd = q & 1u, high = q & 2u;
+    const float low = (odd ? v[1] : v[0]) + ovl_lane::quad_xor1(odd ? v[0] : v[1]);
+    const float up = (odd ? v[3] : v[2]) + ovl_lane::quad_xor1(odd ? v[2] : v[3]);
+    return (high ? up : low) + ovl_lane::quad_xor2(high ? low : up);
+}
+
+// quad_from with a number that is constant once the loops around it are unrolled
+__device__ __forceinline__ float quad_pick(float x, int k) {
+    switch (k) {
+        case 0: return ovl_lane::quad_from<0>(x);
+        case 1: return ovl_lane::quad_from<1>(x);
+        case 2: return ovl_lane::quad_from<2>(x);
+        default: return ovl_lane::quad_from<3>(x);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------------------------------------------------
+
+// OUTPUT: the full pass (y, the last state, the kept states).  Otherwise only states: the chunk's own effect on a zero
+// state (`local`, `dt_sum`), or the kept states.
+template <typename T, int S, bool OUTPUT>
+__global__ void __launch_bounds__(THREADS)
+scan_forward_kernel(scan_args<T> p, uint32_t chunks, T* y, float* last, float* saved, const float* entry, float* local,
+                    float* dt_sum) {
+    constexpr uint32_t NP = 4 * S;
+    __shared__ __attribute__((aligned(16))) float lds_B[2][TILE * NP];
+    __shared__ __attribute__((aligned(16))) float lds_C[OUTPUT ? 2 : 1][OUTPUT ? TILE * NP : 1];
+    const place w = find_place(p, 0u, chunks);
+    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels + w.channel;
+    const uint64_t state_row = (uint64_t)w.b * p.channels + w.channel;
+
+    float h[S], A2[S];
+    load_entries(A2, p.A + (uint64_t)w.channel * p.state, w.q, p.state);
+#pragma unroll
+    for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; h[s] = 0.0f; }
+    if (entry != nullptr) load_states(h, entry + chunk_row * NP + w.q * S);
+    else if (local == nullptr && p.entering != nullptr) load_entries(h, p.entering + state_row * p.state, w.q, p.state);
+    const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
+    const float skip = OUTPUT && p.D != nullptr ? p.D[w.channel] : 0.0f;
+    const bool gate = OUTPUT && p.z.data != nullptr;
+    float dt_total = 0.0f;
+
+    T u_next[QUADS], delta_next[QUADS], z_next[QUADS];
+    vector_stage<T, S> B_next, C_next;
+    auto fetch = [&](uint32_t t0) {
+        load_tile(u_next, p.u, w, t0, p.length);
+        load_tile(delta_next, p.delta, w, t0, p.length);
+        if (gate) load_tile(z_next, p.z, w, t0, p.length);
+        B_next.load(p.B, w, t0, p.length, p.state);
+        if (OUTPUT) C_next.load(p.C, w, t0, p.length, p.state);
+    };
+    if (w.first * TILE < w.end) fetch(w.first * TILE);
+
+    for (uint32_t tile = w.first; tile < w.last; ++tile) {
+        const uint32_t t0 = tile * TILE;
+        if (t0 >= w.end) {                  // behind the sequence: the state stays, the outputs are zero
+            if (OUTPUT && w.active)
+#pragma unroll
+                for (uint32_t j = 0; j < QUADS; ++j) {
+                    const uint32_t t = t0 + 4u * j + w.q;
+                    if (t < p.length) y[((uint64_t)w.b * p.length + t) * p.channels + w.channel] = narrow<T>(0.0f);
+                }
+            continue;
+        }
+        const uint32_t buffer = tile & 1u;
+        B_next.store(lds_B[buffer], w, t0, p.state);
+        if (OUTPUT) C_next.store(lds_C[OUTPUT ? buffer : 0], w, t0, p.state);
+        float u[QUADS], delta[QUADS], z[QUADS];
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+            u[j] = widen<T>(u_next[j]);
+            delta[j] = widen<T>(delta_next[j]) + bias;
+            z[j] = gate ? widen<T>(z_next[j]) : 0.0f;
+        }
+        // One barrier per tile: the buffer written now was last read two tiles ago, and the barrier in between has
+        // let every wavefront finish that tile.
+        __syncthreads();
+        if (tile + 1u < w.last && t0 + TILE < w.end) fetch(t0 + TILE);
+        if (saved != nullptr && w.active)
+            store_states(h, saved + (((uint64_t)w.b * p.tiles + tile) * p.channels + w.channel) * NP + w.q * S);
+
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+            const uint32_t t = t0 + 4u * j + w.q;
+            const bool token = t < w.end;
+            const float dt = token ? (p.softplus ? softplus_(delta[j]) : delta[j]) : 0.0f;
+            const float uu = token ? u[j] : 0.0f;
+            const float x = dt * uu;
+            dt_total += dt;
+            float part[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float* Bt = lds_B[buffer] + (4u * j + k) * NP + w.q * S;
+                const float* Ct = lds_C[OUTPUT ? buffer : 0] + (OUTPUT ? (4u * j + k) * NP + w.q * S : 0u);
+                const float dt_k = quad_pick(dt, k), x_k = quad_pick(x, k);
+                float sum = 0.0f;
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    const float a = ovl_lane::exp2_(dt_k * A2[s]);
+                    h[s] = fmaf(a, h[s], x_k * Bt[s]);
+                    if (OUTPUT) sum = fmaf(Ct[s], h[s], sum);
+                }
+                part[k] = sum;
+            }
+            if (OUTPUT) {
+                float out = fmaf(skip, uu, quad_scatter_sum(part, w.q));
+                if (gate) out *= z[j] * sigmoid_(z[j]);
+                if (w.active && t < p.length)
+                    y[((uint64_t)w.b * p.length + t) * p.channels + w.channel] = narrow<T>(token ? out : 0.0f);
+            }
+        }
+    }
+    if (OUTPUT && w.active && w.chunk + 1u == p.chunks) store_entries(h, last + state_row * p.state, w.q, p.state);
+    if (!OUTPUT && local != nullptr) {
+        dt_total = quad_sum(dt_total);
+        if (w.active) {
+            store_states(h, local + chunk_row * NP + w.q * S);
+            if (w.q == 0u) dt_sum[chunk_row] = dt_total;
+        }
+    }
+}
+
+// Joins the chunks: in place of each chunk's own effect `local` the state that enters it.  One thread per (sequence,
+// channel, state entry).  REVERSE: the gradient's recurrence, which enters chunks from their ends.  Eight chunks are read
+// before they are overwritten, so that the loads do not wait for one another.
+template <bool REVERSE>
+__global__ void __launch_bounds__(THREADS)
+scan_join_kernel(const float* A, const float* start, float* local, const float* dt_sum, uint32_t batch, uint32_t channels,
+                 uint32_t state, uint32_t padded, uint32_t chunks) {
+    const uint64_t id = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
+    if (id >= (uint64_t)batch * channels * padded) return;
+    const uint32_t n = (uint32_t)(id % padded);
+    const uint64_t row = id / padded;
+    const uint32_t channel = (uint32_t)(row % channels), b = (uint32_t)(row / channels);
+    const bool real = n < state;
+    const float A2 = real ? A[(uint64_t)channel * state + n] * LOG2E : 0.0f;
+    float h = real && start != nullptr ? start[row * state + n] : 0.0f;
+    constexpr uint32_t AHEAD = 8;
+    for (uint32_t base = 0; base < chunks; base += AHEAD) {
+        float own[AHEAD], sum[AHEAD];
+        uint64_t at[AHEAD];
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t step = min(base + i, chunks - 1u);
+            const uint32_t chunk = REVERSE ? chunks - 1u - step : step;
+            at[i] = ((uint64_t)b * chunks + chunk) * channels + channel;
+            // the last chunk of the walk has no effect to pass on (and none was computed)
+            const bool passes = step + 1u < chunks;
+            own[i] = passes ? local[at[i] * padded + n] : 0.0f;
+            sum[i] = passes ? dt_sum[at[i]] : 0.0f;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+            if (base + i < chunks) {
+                local[at[i] * padded + n] = h;
+                h = fmaf(ovl_lane::exp2_(sum[i] * A2), h, own[i]);
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------------------------------------------------
+
+template <typename T> struct gradient_args {
+    sequence<T> d_y;
+    const float* d_last;
+    T *d_u, *d_delta, *d_z;
+    float* d_entering;
+    // parts that a later kernel sums: dB and dC per block of channels, dA, dD and d_bias per sequence and chunk
+    float *vector_part, *A_part, *D_part, *bias_part;
+};
+
+// The upstream gradient of y before the gate.
+__device__ __forceinline__ float gated(float d_out, bool gate, float z) { return gate ? d_out * z * sigmoid_(z) : d_out; }
+
+// The effect of a chunk on a zero gradient entering at its end: r = a (C dy + r), tokens walked from the last.
+template <typename T, int S>
+__global__ void __launch_bounds__(THREADS)
+scan_gradient_local_kernel(scan_args<T> p, sequence<T> d_y, float* local, float* dt_sum) {
+    constexpr uint32_t NP = 4 * S;
+    __shared__ __attribute__((aligned(16))) float lds_C[2][TILE * NP];
+    const place w = find_place(p, 1u, p.chunks - 1u);       // nothing enters from the first chunk
+    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels + w.channel;
+    float r[S], A2[S];
+    load_entries(A2, p.A + (uint64_t)w.channel * p.state, w.q, p.state);
+#pragma unroll
+    for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; r[s] = 0.0f; }
+    const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
+    const bool gate = p.z.data != nullptr;
+    float dt_total = 0.0f;
+
+    T delta_next[QUADS], z_next[QUADS], dy_next[QUADS];
+    vector_stage<T, S> C_next;
+    auto fetch = [&](uint32_t t0) {
+        load_tile(delta_next, p.delta, w, t0, p.length);
+        load_tile(dy_next, d_y, w, t0, p.length);
+        if (gate) load_tile(z_next, p.z, w, t0, p.length);
+        C_next.load(p.C, w, t0, p.length, p.state);
+    };
+    const uint32_t stop = min(w.last, (w.end + TILE - 1u) / TILE);
+    if (w.first < stop) fetch((stop - 1u) * TILE);
+    for (uint32_t tile = stop; tile-- > w.first;) {
+        const uint32_t t0 = tile * TILE, buffer = tile & 1u;
+        C_next.store(lds_C[buffer], w, t0, p.state);
+        float delta[QUADS], dy[QUADS];
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+            delta[j] = widen<T>(delta_next[j]) + bias;
+            dy[j] = gated(widen<T>(dy_next[j]), gate, gate ? widen<T>(z_next[j]) : 0.0f);
+        }
+        __syncthreads();
+        if (tile > w.first) fetch(t0 - TILE);
+#pragma unroll
+        for (uint32_t i = 0; i < QUADS; ++i) {
+            const uint32_t j = QUADS - 1u - i;
+            const bool token = t0 + 4u * j + w.q < w.end;
+            const float dt = token ? (p.softplus ? softplus_(delta[j]) : delta[j]) : 0.0f;
+            const float d = token ? dy[j] : 0.0f;
+            dt_total += dt;
+#pragma unroll
+            for (int k = 3; k >= 0; --k) {
+                const float* Ct = lds_C[buffer] + (4u * j + k) * NP + w.q * S;
+                const float dt_k = quad_pick(dt, k), d_k = quad_pick(d, k);
+#pragma unroll
+                for (int s = 0; s < S; ++s) r[s] = ovl_lane::exp2_(dt_k * A2[s]) * fmaf(d_k, Ct[s], r[s]);
+            }
+        }
+    }
+    dt_total = quad_sum(dt_total);
+    if (w.active) {
+        store_states(r, local + chunk_row * NP + w.q * S);
+        if (w.q == 0u) dt_sum[chunk_row] = dt_total;
+    }
+}
+
+// Sums over the 16 channels of a wavefront (the quads) of 2 S values per lane and token, four tokens together.  Within a
+// row every addition halves the number of values a lane holds: afterwards quad i of a row holds entries
+// m + (S / 2) (i & 1) of the first (i < 2) or second set; the rows then trade tokens: row r ends with token r.
+template <int S> struct channel_sums {
+    static constexpr int KEPT = S >= 2 ? S / 2 : 1;
+    float kept[KEPT][4];
+    __device__ __forceinline__ void add(const float (&first)[S], const float (&second)[S], int k, uint32_t lane) {
+        const bool far = lane & 8u, odd = lane & 4u;
+        float v[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const float a = first[s] + ovl_lane::row_round<8>(first[s]), b = second[s] + ovl_lane::row_round<8>(second[s]);
+            v[s] = far ? b : a;
+        }
+        if constexpr (S == 1) {
+            kept[0][k] = v[0] + (odd ? ovl_lane::row_up<4>(v[0]) : ovl_lane::row_down<4>(v[0]));
+        } else {
+#pragma unroll
+            for (int m = 0; m < S / 2; ++m) {
+                const float a = v[m] + ovl_lane::row_down<4>(v[m]), b = v[m + S / 2] + ovl_lane::row_up<4>(v[m + S / 2]);
+                kept[m][k] = odd ? b : a;
+            }
+        }
+    }
+    // Writes the sums to lds [2][TILE][NP] for the four tokens from `t`.
+    __device__ __forceinline__ void put(float* lds, uint32_t t, uint32_t lane) {
+        constexpr uint32_t NP = 4 * S;
+        const uint32_t row = lane / 16u, quad = (lane / 4u) & 3u, q = lane & 3u;
+#pragma unroll
+        for (int m = 0; m < KEPT; ++m) {
+            float a = kept[m][0], b = kept[m][1], c = kept[m][2], d = kept[m][3];
+            ovl_lane::swap_halves(a, c);
+            ovl_lane::swap_halves(b, d);
+            float even = a + c, odd = b + d;
+            ovl_lane::swap_rows(even, odd);
+            const uint32_t s = S == 1 ? 0u : m + (S / 2) * (quad & 1u);
+            lds[((quad >> 1) * TILE + t + row) * NP + q * S + s] = even + odd;
+        }
+    }
+};
+
+template <typename T, int S>
+__global__ void __launch_bounds__(THREADS)
+scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, const float* entry) {
+    constexpr uint32_t NP = 4 * S;
+    // tokens whose states and decays are held in registers at a time
+    constexpr uint32_t SUB = S <= 4 ? 16 : S <= 8 ? 8 : 4, SUBS = TILE / SUB;
+    __shared__ __attribute__((aligned(16))) float lds_B[2][TILE * NP];
+    __shared__ __attribute__((aligned(16))) float lds_C[2][TILE * NP];
+    __shared__ float lds_sums[WAVES][2 * TILE * NP];
+    const place w = find_place(p, 0u, p.chunks);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u;
+    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels + w.channel;
+    const uint64_t state_row = (uint64_t)w.b * p.channels + w.channel;
+
+    float r[S], A2[S], dA[S];
+    load_entries(A2, p.A + (uint64_t)w.channel * p.state, w.q, p.state);
+#pragma unroll
+    for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; r[s] = 0.0f; dA[s] = 0.0f; }
+    if (entry != nullptr) load_states(r, entry + chunk_row * NP + w.q * S);
+    else if (g.d_last != nullptr) load_entries(r, g.d_last + state_row * p.state, w.q, p.state);
+    const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
+    const float skip = p.D != nullptr ? p.D[w.channel] : 0.0f;
+    const bool gate = p.z.data != nullptr;
+    float dD = 0.0f, dbias = 0.0f;
+
+    T u_next[QUADS], delta_next[QUADS], z_next[QUADS], dy_next[QUADS];
+    float h_next[S];
+    vector_stage<T, S> B_next, C_next;
+    auto fetch = [&](uint32_t tile) {
+        const uint32_t t0 = tile * TILE;
+        load_tile(u_next, p.u, w, t0, p.length);
+        load_tile(delta_next, p.delta, w, t0, p.length);
+        load_tile(dy_next, g.d_y, w, t0, p.length);
+        if (gate) load_tile(z_next, p.z, w, t0, p.length);
+        load_states(h_next, saved + (((uint64_t)w.b * p.tiles + tile) * p.channels + w.channel) * NP + w.q * S);
+        B_next.load(p.B, w, t0, p.length, p.state);
+        C_next.load(p.C, w, t0, p.length, p.state);
+    };
+    const uint32_t stop = max(w.first, min(w.last, (w.end + TILE - 1u) / TILE));
+    float* const part = g.vector_part + (((uint64_t)w.g * p.blocks + w.block) * p.batch + w.b) * p.length * (2u * p.state);
+
+    // behind the sequence all gradients are zero
+    for (uint32_t t = stop * TILE + threadIdx.x / BLOCK; t < min(w.last * TILE, p.length); t += THREADS / BLOCK) {
+        const uint32_t c = w.block * BLOCK + threadIdx.x % BLOCK;
+        if (c < p.per_group) {
+            const uint64_t at = ((uint64_t)w.b * p.length + t) * p.channels + w.g * p.per_group + c;
+            g.d_u[at] = narrow<T>(0.0f);
+            g.d_delta[at] = narrow<T>(0.0f);
+            if (gate) g.d_z[at] = narrow<T>(0.0f);
+        }
+        for (uint32_t n = threadIdx.x % BLOCK; n < 2u * p.state; n += BLOCK) part[(uint64_t)t * 2u * p.state + n] = 0.0f;
+    }
+
+    if (w.first < stop) fetch(stop - 1u);
+    for (uint32_t tile = stop; tile-- > w.first;) {
+        const uint32_t t0 = tile * TILE, buffer = tile & 1u;
+        B_next.store(lds_B[buffer], w, t0, p.state);
+        C_next.store(lds_C[buffer], w, t0, p.state);
+        float u[QUADS], raw[QUADS], dt[QUADS], x[QUADS], z[QUADS], d_out[QUADS], d[QUADS], h[SUBS][S];
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+            const bool token = t0 + 4u * j + w.q < w.end;
+            u[j] = token ? widen<T>(u_next[j]) : 0.0f;
+            raw[j] = widen<T>(delta_next[j]) + bias;
+            dt[j] = token ? (p.softplus ? softplus_(raw[j]) : raw[j]) : 0.0f;
+            x[j] = dt[j] * u[j];
+            z[j] = gate ? widen<T>(z_next[j]) : 0.0f;
+            d_out[j] = token ? widen<T>(dy_next[j]) : 0.0f;
+            d[j] = token ? gated(d_out[j], gate, z[j]) : 0.0f;
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[0][s] = h_next[s];
+        // also lets every wavefront finish reading lds_sums of the tile before
+        __syncthreads();
+        if (tile > w.first) fetch(tile - 1u);
+
+        // the states that enter the later parts of the tile
+#pragma unroll
+        for (uint32_t part_of = 0; part_of + 1u < SUBS; ++part_of) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) h[part_of + 1u][s] = h[part_of][s];
+#pragma unroll
+            for (uint32_t i = 0; i < SUB; ++i) {
+                const uint32_t at = part_of * SUB + i;
+                const float* Bt = lds_B[buffer] + at * NP + w.q * S;
+                const float dt_k = quad_pick(dt[at / 4u], at & 3u), x_k = quad_pick(x[at / 4u], at & 3u);
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+                    h[part_of + 1u][s] = fmaf(ovl_lane::exp2_(dt_k * A2[s]), h[part_of + 1u][s], x_k * Bt[s]);
+            }
+        }
+
+        float dA_tile[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) dA_tile[s] = 0.0f;
+#pragma unroll
+        for (uint32_t back = 0; back < SUBS; ++back) {
+            const uint32_t part_of = SUBS - 1u - back;
+            float a[SUB][S], state[SUB + 1u][S], y[SUB / 4u];
+#pragma unroll
+            for (int s = 0; s < S; ++s) state[0][s] = h[part_of][s];
+#pragma unroll
+            for (uint32_t i = 0; i < SUB; i += 4u) {
+                const uint32_t j = part_of * (SUB / 4u) + i / 4u;
+                float sums[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float* Bt = lds_B[buffer] + (4u * j + k) * NP + w.q * S;
+                    const float* Ct = lds_C[buffer] + (4u * j + k) * NP + w.q * S;
+                    const float dt_k = quad_pick(dt[j], k), x_k = quad_pick(x[j], k);
+                    sums[k] = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < S; ++s) {
+                        a[i + k][s] = ovl_lane::exp2_(dt_k * A2[s]);
+                        state[i + k + 1][s] = fmaf(a[i + k][s], state[i + k][s], x_k * Bt[s]);
+                        if (gate) sums[k] = fmaf(Ct[s], state[i + k + 1][s], sums[k]);
+                    }
+                }
+                y[i / 4u] = gate ? fmaf(skip, u[j], quad_scatter_sum(sums, w.q)) : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t step = 0; step < SUB; step += 4u) {
+                const uint32_t i = SUB - 4u - step, j = part_of * (SUB / 4u) + i / 4u;
+                channel_sums<S> sums;
+                float dx[4], through[4];
+#pragma unroll
+                for (int k = 3; k >= 0; --k) {
+                    const float* Bt = lds_B[buffer] + (4u * j + k) * NP + w.q * S;
+                    const float* Ct = lds_C[buffer] + (4u * j + k) * NP + w.q * S;
+                    const float dt_k = quad_pick(dt[j], k), x_k = quad_pick(x[j], k), d_k = quad_pick(d[j], k);
+                    float dB[S], dC[S];
+                    dx[k] = 0.0f;
+                    through[k] = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < S; ++s) {
+                        const float grad = fmaf(d_k, Ct[s], r[s]);
+                        dx[k] = fmaf(grad, Bt[s], dx[k]);
+                        dB[s] = grad * x_k;
+                        dC[s] = d_k * state[i + k + 1][s];
+                        r[s] = grad * a[i + k][s];
+                        const float moved = r[s] * state[i + k][s];
+                        dA_tile[s] = fmaf(dt_k, moved, dA_tile[s]);
+                        through[k] = fmaf(moved, A2[s], through[k]);
+                    }
+                    // lanes without a channel add nothing
+#pragma unroll
+                    for (int s = 0; s < S; ++s) { dB[s] = w.active ? dB[s] : 0.0f; dC[s] = w.active ? dC[s] : 0.0f; }
+                    sums.add(dB, dC, k, lane);
+                }
+                sums.put(lds_sums[wave], 4u * j, lane);
+                const uint32_t t = t0 + 4u * j + w.q;
+                const bool token = t < w.end;
+                const float d_x = quad_scatter_sum(dx, w.q);
+                float d_dt = fmaf(d_x, u[j], LN2 * quad_scatter_sum(through, w.q));
+                if (p.softplus) d_dt *= sigmoid_(raw[j]);
+                d_dt = token ? d_dt : 0.0f;
+                dbias += d_dt;
+                dD = fmaf(d[j], u[j], dD);
+                if (w.active && t < p.length) {
+                    const uint64_t at = ((uint64_t)w.b * p.length + t) * p.channels + w.channel;
+                    g.d_u[at] = narrow<T>(token ? fmaf(d_x, dt[j], skip * d[j]) : 0.0f);
+                    g.d_delta[at] = narrow<T>(d_dt);
+                    if (gate) {
+                        const float s = sigmoid_(z[j]);
+                        g.d_z[at] = narrow<T>(token ? d_out[j] * y[i / 4u] * s * fmaf(z[j], 1.0f - s, 1.0f) : 0.0f);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) dA[s] += dA_tile[s];
+
+        // the four wavefronts' sums, as [token][B entries, C entries]
+        __syncthreads();
+        for (uint32_t at = threadIdx.x; at < 2u * TILE * NP; at += THREADS) {
+            const uint32_t set = at / (TILE * NP), t = at / NP % TILE, n = at % NP;
+            if (n < p.state && t0 + t < p.length) {
+                float sum = 0.0f;
+#pragma unroll
+                for (uint32_t v = 0; v < WAVES; ++v) sum += lds_sums[v][at];
+                part[(uint64_t)(t0 + t) * 2u * p.state + set * p.state + n] = t0 + t < w.end ? sum : 0.0f;
+            }
+        }
+    }
+    if (w.active) {
+        store_states(dA, g.A_part + chunk_row * NP + w.q * S);
+        if (w.chunk == 0u && g.d_entering != nullptr) store_entries(r, g.d_entering + state_row * p.state, w.q, p.state);
+    }
+    dD = quad_sum(dD);
+    dbias = quad_sum(dbias);
+    if (w.active && w.q == 0u) {
+        g.D_part[chunk_row] = dD;
+        g.bias_part[chunk_row] = dbias;
+    }
+}
+
+// Sums the parts of dB and dC over the blocks of a group, and of dA, dD and d_bias over sequences and chunks.  One thread
+// per result; the order of the additions is fixed.
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+scan_gradient_sum_kernel(const float* vector_part, const float* A_part, const float* D_part, const float* bias_part,
+                         uint32_t batch, uint32_t length, uint32_t channels, uint32_t state, uint32_t padded,
+                         uint32_t groups, uint32_t blocks, uint32_t rows, uint32_t vector_groups,
+                         T* d_B, T* d_C, float* d_A, float* d_D, float* d_bias) {
+    const uint64_t per_block = (uint64_t)batch * length * 2u * state;
+    if (blockIdx.x < vector_groups) {
+        const uint64_t id = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
+        if (id >= per_block * groups) return;
+        const uint32_t g = (uint32_t)(id / per_block);
+        const uint64_t in = id % per_block;
+        const float* from = vector_part + (uint64_t)g * blocks * per_block + in;
+        float sum = 0.0f;
+#pragma unroll 8
+        for (uint32_t k = 0; k < blocks; ++k) sum += from[k * per_block];
+        const uint32_t n = (uint32_t)(in % (2u * state));
+        const uint64_t token = in / (2u * state);
+        T* to = n < state ? d_B : d_C;
+        to[(token * groups + g) * state + (n < state ? n : n - state)] = narrow<T>(sum);
+        return;
+    }
+    // then state + 2 results per channel: dA, dD, d_bias
+    const uint64_t id = (uint64_t)(blockIdx.x - vector_groups) * THREADS + threadIdx.x;
+    const uint32_t n = (uint32_t)(id % (state + 2u));
+    const uint64_t channel = id / (state + 2u);
+    if (channel >= channels) return;
+    float sum = 0.0f;
+    if (n < state) {
+#pragma unroll 8
+        for (uint32_t k = 0; k < rows; ++k) sum += A_part[((uint64_t)k * channels + channel) * padded + n];
+        d_A[channel * state + n] = sum;
+    } else if ((n == state ? d_D : d_bias) != nullptr) {
+        const float* from = n == state ? D_part : bias_part;
+#pragma unroll 8
+        for (uint32_t k = 0; k < rows; ++k) sum += from[(uint64_t)k * channels + channel];
+        (n == state ? d_D : d_bias)[channel] = sum;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// one token
+// ---------------------------------------------------------------------------------------------------------------------
+
+// The recurrence once: a quad per (sequence, channel), as above.  Bound by reading and writing the state.
+template <typename T, int S, bool WHOLE>
+__global__ void __launch_bounds__(THREADS)
+scan_step_kernel(scan_args<T> p, float* state, int64_t state_stride, T* y) {
+    const uint64_t id = ((uint64_t)blockIdx.x * THREADS + threadIdx.x) / 4u, every = (uint64_t)p.batch * p.channels;
+    const uint32_t q = threadIdx.x & 3u;
+    const bool active = id < every;
+    const uint32_t b = (uint32_t)((active ? id : every - 1u) / p.channels);
+    const uint32_t channel = (uint32_t)((active ? id : every - 1u) % p.channels);
+    float* own = state + (int64_t)b * state_stride + (uint64_t)channel * p.state;
+    const float* A = p.A + (uint64_t)channel * p.state;
+    const T* B = p.B.data + (int64_t)b * p.B.batch_stride + (int64_t)(channel / p.per_group) * p.B.group_stride;
+    const T* C = p.C.data + (int64_t)b * p.C.batch_stride + (int64_t)(channel / p.per_group) * p.C.group_stride;
+    float h[S], A_row[S], B_row[S], C_row[S];
+    if constexpr (WHOLE) {                  // all of 4 S entries, S of them 16-byte aligned or a whole vector
+        typedef float vec __attribute__((ext_vector_type(S >= 4 ? 4 : S)));
+        constexpr int PIECES = S >= 4 ? S / 4 : 1, WIDE = S >= 4 ? 4 : S;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const vec v = *reinterpret_cast<const vec*>(own + q * S + i * WIDE);
+            const vec a = *reinterpret_cast<const vec*>(A + q * S + i * WIDE);
+#pragma unroll
+            for (int k = 0; k < WIDE; ++k) { h[i * WIDE + k] = v[k]; A_row[i * WIDE + k] = a[k]; }
+        }
+    } else {
+        load_entries(h, own, q, p.state);
+        load_entries(A_row, A, q, p.state);
+    }
+#pragma unroll
+    for (uint32_t s = 0; s < S; ++s) {
+        const uint32_t at = min(q * S + s, p.state - 1u);
+        B_row[s] = q * S + s < p.state ? widen<T>(B[at]) : 0.0f;
+        C_row[s] = q * S + s < p.state ? widen<T>(C[at]) : 0.0f;
+    }
+    const float u = widen<T>(p.u.data[(int64_t)b * p.u.batch_stride + channel]);
+    float dt = widen<T>(p.delta.data[(int64_t)b * p.delta.batch_stride + channel]);
+    const bool gate = p.z.data != nullptr;
+    const float z = gate ? widen<T>(p.z.data[(int64_t)b * p.z.batch_stride + channel]) : 0.0f;
+    if (p.delta_bias != nullptr) dt += p.delta_bias[channel];
+    if (p.softplus) dt = softplus_(dt);
+    const float x = dt * u;
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        h[s] = fmaf(ovl_lane::exp2_(dt * (A_row[s] * LOG2E)), h[s], x * B_row[s]);
+        sum = fmaf(C_row[s], h[s], sum);
+    }
+    sum = quad_sum(sum);
+    if (p.D != nullptr) sum = fmaf(p.D[channel], u, sum);
+    if (gate) sum *= z * sigmoid_(z);
+    if (!active) return;
+    if constexpr (WHOLE) {
+        typedef float vec __attribute__((ext_vector_type(S >= 4 ? 4 : S)));
+        constexpr int PIECES = S >= 4 ? S / 4 : 1, WIDE = S >= 4 ? 4 : S;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            vec v;
+#pragma unroll
+            for (int k = 0; k < WIDE; ++k) v[k] = h[i * WIDE + k];
+            *reinterpret_cast<vec*>(own + q * S + i * WIDE) = v;
+        }
+    } else {
+        store_entries(h, own, q, p.state);
+    }
+    if (q == 0u) y[id] = narrow<T>(sum);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------------
+
+using ovl_ssm::after_launch;
+using ovl_ssm::fail;
+using ovl_ssm::round_up;
+
+// State entries per lane of a quad: the smallest variant that holds the state.
+uint32_t entries_of(uint32_t state) { return state <= 8u ? 2u : state <= 16u ? 4u : state <= 32u ? 8u : 16u; }
+
+struct plan {
+    uint32_t per_group, blocks, tiles, chunks, chunk_tiles, entries;
+    uint64_t strands;                       // workgroups without a split
+};
+
+// Into how many chunks the length is split.
+void chunks_for(plan& p) {
+    constexpr uint64_t ENOUGH = 192, WANTED = 1024;
+    constexpr uint32_t SHORTEST = 4;        // tiles per chunk
+    p.chunks = 1;
+    if (p.strands < ENOUGH) {
+        const uint64_t wanted = (WANTED + p.strands - 1) / p.strands;
+        const uint32_t most = p.tiles / SHORTEST;
+        p.chunks = (uint32_t)(wanted < most ? wanted : most);
+        if (p.chunks < 3u) p.chunks = 1;
+    }
+    p.chunk_tiles = (p.tiles + p.chunks - 1u) / p.chunks;
+    p.chunks = (p.tiles + p.chunk_tiles - 1u) / p.chunk_tiles;
+}
+
+// Checks a scan; `token` for the one-token form.
+int check(const char* who, const ovl_ssm_scan* s, bool token, plan& p) {
+    const std::string name(who);
+    if (s == nullptr) return fail(OVL_SSM_EINVAL, name + ": null scan");
+    if (s->batch == 0 || s->length == 0 || s->channels == 0 || s->state == 0 || s->groups == 0)
+        return fail(OVL_SSM_EINVAL, name + ": sizes must be positive");
+    if (s->state > 64u) return fail(OVL_SSM_EINVAL, name + ": at most 64 state entries per channel");
+    if (s->channels % s->groups != 0u) return fail(OVL_SSM_EINVAL, name + ": groups must divide channels");
+    if (s->dtype != OVL_SSM_FLOAT16 && s->dtype != OVL_SSM_FLOAT32 && s->dtype != OVL_SSM_BFLOAT16)
+        return fail(OVL_SSM_EINVAL, name + ": unknown element type");
+    if (s->u.data == nullptr || s->delta.data == nullptr || s->B.data == nullptr || s->C.data == nullptr || s->A == nullptr)
+        return fail(OVL_SSM_EINVAL, name + ": null tensor");
+    if (token && (s->length != 1u || s->lengths != nullptr))
+        return fail(OVL_SSM_EINVAL, name + ": a step takes one token of every sequence");
+    if (s->length > (1u << 30)) return fail(OVL_SSM_EINVAL, name + ": length must be at most 2^30");
+    p.entries = entries_of(s->state);
+    p.per_group = s->channels / s->groups;
+    p.blocks = (p.per_group + BLOCK - 1u) / BLOCK;
+    p.tiles = (s->length + TILE - 1u) / TILE;
+    p.strands = (uint64_t)s->batch * s->groups * p.blocks;
+    chunks_for(p);
+    // every launch has at most 2^31 - 1 workgroups
+    const uint64_t most = (1ull << 31) - 1;
+    const uint64_t rows = (uint64_t)s->batch * s->channels;
+    if (p.strands * p.chunks > most || rows * 4u * p.entries / THREADS + 1u > most ||
+        (uint64_t)s->batch * s->length * s->groups * 2u * s->state / THREADS + 1u > most / 2u)
+        return fail(OVL_SSM_EINVAL, name + ": too many elements for one launch");
+    return OVL_SSM_OK;
+}
+
+template <typename T>
+scan_args<T> make_args(const ovl_ssm_scan* s, const plan& p) {
+    auto seq = [](const ovl_ssm_sequence& v) {
+        return sequence<T>{static_cast<const T*>(v.data), v.batch_stride, v.token_stride};
+    };
+    auto vec = [](const ovl_ssm_vectors& v) {
+        return vectors<T>{static_cast<const T*>(v.data), v.batch_stride, v.token_stride, v.group_stride};
+    };
+    return scan_args<T>{s->batch, s->length, s->channels, s->state, s->groups, p.per_group, p.blocks, p.tiles, p.chunks,
+                        p.chunk_tiles, s->softplus, seq(s->u), seq(s->delta), seq(s->z), vec(s->B), vec(s->C), s->A, s->D,
+                        s->delta_bias, s->entering, s->lengths};
+}
+
+// Scratch memory, in floats: the chunks' states and sums of dt; for the backward pass also the parts of the gradients.
+struct layout {
+    uint64_t local, dt_sum, vector_part, A_part, D_part, bias_part, all;
+};
+layout lay_out(const ovl_ssm_scan* s, const plan& p, bool backward) {
+    layout at;
+    const uint64_t rows = (uint64_t)s->batch * p.chunks * s->channels, padded = 4u * p.entries;
+    uint64_t next = 0;
+    auto take = [&](uint64_t n) { const uint64_t here = next; next += round_up(n, 64); return here; };
+    at.local = take(p.chunks > 1u ? rows * padded : 0);
+    at.dt_sum = take(p.chunks > 1u ? rows : 0);
+    at.vector_part = take(backward ? (uint64_t)s->groups * p.blocks * s->batch * s->length * 2u * s->state : 0);
+    at.A_part = take(backward ? rows * padded : 0);
+    at.D_part = take(backward ? rows : 0);
+    at.bias_part = take(backward ? rows : 0);
+    at.all = next;
+    return at;
+}
+
+template <bool REVERSE>
+void join(const ovl_ssm_scan* s, const plan& p, const float* start, float* local, const float* dt_sum, hipStream_t stream) {
+    const uint64_t all = (uint64_t)s->batch * s->channels * 4u * p.entries;
+    hipLaunchKernelGGL((scan_join_kernel<REVERSE>), dim3((uint32_t)((all + THREADS - 1) / THREADS)), dim3(THREADS), 0, stream,
+                       s->A, start, local, dt_sum, s->batch, s->channels, s->state, 4u * p.entries, p.chunks);
+}
+
+template <typename T, int S>
+void forward(const ovl_ssm_scan* s, const plan& p, T* y, float* last, float* saved, float* scratch, hipStream_t stream) {
+    const scan_args<T> args = make_args<T>(s, p);
+    const layout at = lay_out(s, p, false);
+    const float* entry = nullptr;
+    if (p.chunks > 1u) {
+        float* local = scratch + at.local;
+        float* dt_sum = scratch + at.dt_sum;
+        hipLaunchKernelGGL((scan_forward_kernel<T, S, false>), dim3((uint32_t)(p.strands * (p.chunks - 1u))), dim3(THREADS), 0,
+                           stream, args, p.chunks - 1u, static_cast<T*>(nullptr), static_cast<float*>(nullptr),
+                           static_cast<float*>(nullptr), static_cast<const float*>(nullptr), local, dt_sum);
+        join<false>(s, p, s->entering, local, dt_sum, stream);
+        entry = local;
+    }
+    const dim3 grid((uint32_t)(p.strands * p.chunks));
+    if (y != nullptr)
+        hipLaunchKernelGGL((scan_forward_kernel<T, S, true>), grid, dim3(THREADS), 0, stream, args, p.chunks, y, last, saved,
+                           entry, static_cast<float*>(nullptr), static_cast<float*>(nullptr));
+    else
+        hipLaunchKernelGGL((scan_forward_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, p.chunks, y, last, saved,
+                           entry, static_cast<float*>(nullptr), static_cast<float*>(nullptr));
+}
+
+template <typename T, int S>
+void backward(const ovl_ssm_scan* s, const plan& p, const float* saved, const ovl_ssm_scan_gradients* g, float* scratch,
+              hipStream_t stream) {
+    const scan_args<T> args = make_args<T>(s, p);
+    const layout at = lay_out(s, p, true);
+    gradient_args<T> to;
+    to.d_y = sequence<T>{static_cast<const T*>(g->d_y.data), g->d_y.batch_stride, g->d_y.token_stride};
+    to.d_last = g->d_last;
+    to.d_u = static_cast<T*>(g->d_u);
+    to.d_delta = static_cast<T*>(g->d_delta);
+    to.d_z = static_cast<T*>(g->d_z);
+    to.d_entering = g->d_entering;
+    to.vector_part = scratch + at.vector_part;
+    to.A_part = scratch + at.A_part;
+    to.D_part = scratch + at.D_part;
+    to.bias_part = scratch + at.bias_part;
+    const float* entry = nullptr;
+    if (p.chunks > 1u) {
+        float* local = scratch + at.local;
+        float* dt_sum = scratch + at.dt_sum;
+        hipLaunchKernelGGL((scan_gradient_local_kernel<T, S>), dim3((uint32_t)(p.strands * (p.chunks - 1u))), dim3(THREADS), 0,
+                           stream, args, to.d_y, local, dt_sum);
+        join<true>(s, p, g->d_last, local, dt_sum, stream);
+        entry = local;
+    }
+    hipLaunchKernelGGL((scan_backward_kernel<T, S>), dim3((uint32_t)(p.strands * p.chunks)), dim3(THREADS), 0, stream, args, to,
+                       saved, entry);
+    const uint64_t vector_all = (uint64_t)s->groups * s->batch * s->length * 2u * s->state;
+    const uint32_t vector_groups = (uint32_t)((vector_all + THREADS - 1) / THREADS);
+    const uint32_t rest = (uint32_t)(((uint64_t)s->channels * (s->state + 2u) + THREADS - 1) / THREADS);
+    hipLaunchKernelGGL((scan_gradient_sum_kernel<T>), dim3(vector_groups + rest), dim3(THREADS), 0, stream, to.vector_part,
+                       to.A_part, to.D_part, to.bias_part, s->batch, s->length, s->channels, s->state, 4u * p.entries,
+                       s->groups, p.blocks, s->batch * p.chunks, vector_groups, static_cast<T*>(g->d_B),
+                       static_cast<T*>(g->d_C), g->d_A, g->d_D, g->d_delta_bias);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, int S>
+void step(const ovl_ssm_scan* s, const plan& p, float* h, int64_t stride, T* y, hipStream_t stream) {
+    const scan_args<T> args = make_args<T>(s, p);
+    const uint64_t lanes = (uint64_t)s->batch * s->channels * 4u;
+    const dim3 grid((uint32_t)((lanes + THREADS - 1) / THREADS));
+    const bool whole = s->state == 4u * S && aligned16(h) && aligned16(s->A) && stride % 4 == 0;
+    if (whole) hipLaunchKernelGGL((scan_step_kernel<T, S, true>), grid, dim3(THREADS), 0, stream, args, h, stride, y);
+    else hipLaunchKernelGGL((scan_step_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, h, stride, y);
+}
+
+// Calls F<T, S>(...) for the scan's element type and state.
+#define OVL_SSM_BY_STATE(F, T, ...)                          \
+    switch (p.entries) {                                     \
+        case 2u: F<T, 2>(__VA_ARGS__); break;                \
+        case 4u: F<T, 4>(__VA_ARGS__); break;                \
+        case 8u: F<T, 8>(__VA_ARGS__); break;                \
+        default: F<T, 16>(__VA_ARGS__); break;               \
+    }
+
+}  // namespace
+
+extern "C" {
+
+uint64_t ovl_ssm_scan_workspace_bytes(const ovl_ssm_scan* s, int32_t backward_pass) {
+    plan p;
+    if (check("ovl_ssm_scan_workspace_bytes", s, false, p) != OVL_SSM_OK) return 0;
+    return lay_out(s, p, backward_pass != 0).all * sizeof(float);
+}
+
+uint64_t ovl_ssm_scan_saved_bytes(const ovl_ssm_scan* s) {
+    plan p;
+    if (check("ovl_ssm_scan_saved_bytes", s, false, p) != OVL_SSM_OK) return 0;
+    return (uint64_t)s->batch * p.tiles * s->channels * 4u * p.entries * sizeof(float);
+}
+
+int ovl_ssm_scan_forward(const ovl_ssm_scan* s, void* y, float* last, float* saved, void* workspace,
+                         uint64_t workspace_bytes, void* hip_stream) {
+    plan p;
+    const int rc = check("ovl_ssm_scan_forward", s, false, p);
+    if (rc != OVL_SSM_OK) return rc;
+    if ((y == nullptr) != (last == nullptr) || (y == nullptr && saved == nullptr))
+        return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_forward: y and last go together; without them saved is needed");
+    const uint64_t need = lay_out(s, p, false).all * sizeof(float);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_forward: workspace too small or not 16-byte aligned");
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    float* scratch = static_cast<float*>(workspace);
+    switch (s->dtype) {
+        case OVL_SSM_FLOAT32: OVL_SSM_BY_STATE(forward, float, s, p, static_cast<float*>(y), last, saved, scratch, stream) break;
+        case OVL_SSM_FLOAT16: OVL_SSM_BY_STATE(forward, f16, s, p, static_cast<f16*>(y), last, saved, scratch, stream) break;
+        default: OVL_SSM_BY_STATE(forward, bf16, s, p, static_cast<bf16*>(y), last, saved, scratch, stream) break;
+    }
+    return after_launch("ovl_ssm_scan_forward");
+}
+
+int ovl_ssm_scan_backward(const ovl_ssm_scan* s, const float* saved, const ovl_ssm_scan_gradients* g, void* workspace,
+                          uint64_t workspace_bytes, void* hip_stream) {
+    plan p;
+    const int rc = check("ovl_ssm_scan_backward", s, false, p);
+    if (rc != OVL_SSM_OK) return rc;
+    if (g == nullptr || saved == nullptr || g->d_y.data == nullptr || g->d_u == nullptr || g->d_delta == nullptr ||
+        g->d_B == nullptr || g->d_C == nullptr || g->d_A == nullptr || (s->z.data != nullptr && g->d_z == nullptr))
+        return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_backward: null tensor");
+    if (workspace == nullptr || workspace_bytes < lay_out(s, p, true).all * sizeof(float) || !aligned16(workspace))
+        return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_backward: workspace too small or not 16-byte aligned");
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    float* scratch = static_cast<float*>(workspace);
+    switch (s->dtype) {
+        case OVL_SSM_FLOAT32: OVL_SSM_BY_STATE(backward, float, s, p, saved, g, scratch, stream) break;
+        case OVL_SSM_FLOAT16: OVL_SSM_BY_STATE(backward, f16, s, p, saved, g, scratch, stream) break;
+        default: OVL_SSM_BY_STATE(backward, bf16, s, p, saved, g, scratch, stream) break;
+    }
+    return after_launch("ovl_ssm_scan_backward");
+}
+
+int ovl_ssm_scan_step(const ovl_ssm_scan* s, float* h, int64_t h_batch_stride, void* y, void* hip_stream) {
+    plan p;
+    const int rc = check("ovl_ssm_scan_step", s, true, p);
+    if (rc != OVL_SSM_OK) return rc;
+    if (h == nullptr || y == nullptr) return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_step: null tensor");
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    switch (s->dtype) {
+        case OVL_SSM_FLOAT32: OVL_SSM_BY_STATE(step, float, s, p, h, h_batch_stride, static_cast<float*>(y), stream) break;
+        case OVL_SSM_FLOAT16: OVL_SSM_BY_STATE(step, f16, s, p, h, h_batch_stride, static_cast<f16*>(y), stream) break;
+        default: OVL_SSM_BY_STATE(step, bf16, s, p, h, h_batch_stride, static_cast<bf16*>(y), stream) break;
+    }
+    return after_launch("ovl_ssm_scan_step");
+}
+
+}  // extern "C"

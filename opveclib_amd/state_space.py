@@ -1,0 +1,591 @@
+"""
+The hand-written state space kernels (``csrc/ovl_ssm_scan.hip``, ``csrc/ovl_ssm_conv.hip``, C ABI in
+``include/ovl_ssm.h``) from Python: the selective state space scan and the short causal convolution in front of it.
+
+Like the row scans (``row_scan``) and the LSTM cell (``lstm_cell``) these are recurrences with run-time shapes: nothing is
+traced, generated or compiled when they are called.  Each comes as a plain call for whole sequences (:func:`scan`,
+:func:`conv`), its gradient (:func:`scan_grad`, :func:`conv_grad`), a differentiable PyTorch function
+(:func:`scan_torch`, :func:`conv_torch`) and a form for one new token per sequence that updates its state in place
+(:func:`scan_step`, :func:`conv_step`).
+
+Sequences are [batch, length, channels] tensors of one type - float32, float16 or bfloat16 - on one HIP device; their
+channels lie side by side, the other strides are free (so halves of a projection are used where they are; a tensor with
+other channel strides is copied first).  States, statistics and gradients of parameters are float32 throughout; outputs
+are rounded once.  Launches go to the current PyTorch HIP stream and do not synchronise; equal calls give equal bits.
+
+``lengths`` ([batch], int32, on the device) says how many tokens of a padded batch belong to each sequence (values are
+clamped to 0 .. length): returned states are those after the last token, outputs and gradients behind it are zero, and
+what the padding holds is not looked at.
+"""
+
+import ctypes
+import os
+import subprocess
+
+from . import local
+
+library_path = os.path.join(local.csrc_directory, 'libovl_ssm.so')
+source_paths = [os.path.join(local.csrc_directory, n) for n in ('ovl_ssm_scan.hip', 'ovl_ssm_conv.hip')]
+include_directory = os.path.normpath(os.path.join(local.csrc_directory, '..', '..', 'include'))
+
+EXPORTED_SYMBOLS = ('ovl_ssm_scan_workspace_bytes', 'ovl_ssm_scan_saved_bytes', 'ovl_ssm_scan_forward',
+                    'ovl_ssm_scan_backward', 'ovl_ssm_scan_step', 'ovl_ssm_conv_forward', 'ovl_ssm_conv_workspace_bytes',
+                    'ovl_ssm_conv_backward', 'ovl_ssm_conv_step', 'ovl_ssm_last_error')
+
+#: largest number of state entries per channel, and of taps of the convolution
+MAX_STATE, MAX_WIDTH = 64, 4
+
+
+def build(force=False):
+    """Compile the library with hipcc next to its sources (same flags as generated operators); returns its path."""
+    from .compiler import HIPCC_FLAGS
+    headers = [os.path.join(local.csrc_directory, n) for n in ('ovl_lane.h', 'ovl_ssm_host.h')]
+    headers.append(os.path.join(include_directory, 'ovl_ssm.h'))
+    newest = max(os.path.getmtime(p) for p in source_paths + headers)
+    if not force and os.path.exists(library_path) and os.path.getmtime(library_path) >= newest:
+        return library_path
+    tag = '.tmp.%d' % os.getpid()
+    flags = [local.hipcc] + [f for f in HIPCC_FLAGS if f != '-shared'] + ['-I' + include_directory,
+                                                                          '-I' + local.csrc_directory]
+    objects = [p[:-len('.hip')] + tag + '.o' for p in source_paths]
+    running = [subprocess.Popen(flags + ['-c', source, '-o', to], stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                universal_newlines=True) for source, to in zip(source_paths, objects)]
+    try:
+        said = [p.communicate()[0] for p in running]
+        if any(p.returncode != 0 for p in running):
+            raise RuntimeError('hipcc failed for the state space library:\n' + '\n'.join(said))
+        try:
+            subprocess.check_output([local.hipcc, '--offload-arch=' + local.gpu_arch, '-shared'] + objects +
+                                    ['-o', library_path + tag], stderr=subprocess.STDOUT, universal_newlines=True)
+        except subprocess.CalledProcessError as exception:
+            raise RuntimeError('hipcc failed for the state space library:\n' + exception.output)
+    finally:
+        for path in objects:
+            if os.path.exists(path):
+                os.remove(path)
+    os.replace(library_path + tag, library_path)
+    return library_path
+
+
+class Sequence(ctypes.Structure):
+    """``ovl_ssm_sequence``"""
+    _fields_ = [('data', ctypes.c_void_p), ('batch_stride', ctypes.c_int64), ('token_stride', ctypes.c_int64)]
+
+
+class Vectors(ctypes.Structure):
+    """``ovl_ssm_vectors``"""
+    _fields_ = [('data', ctypes.c_void_p), ('batch_stride', ctypes.c_int64), ('token_stride', ctypes.c_int64),
+                ('group_stride', ctypes.c_int64)]
+
+
+class Scan(ctypes.Structure):
+    """``ovl_ssm_scan``"""
+    _fields_ = [(n, ctypes.c_uint32) for n in ('batch', 'length', 'channels', 'state', 'groups')] + \
+               [('dtype', ctypes.c_int32), ('softplus', ctypes.c_int32)] + \
+               [(n, Sequence) for n in ('u', 'delta', 'z')] + [(n, Vectors) for n in ('B', 'C')] + \
+               [(n, ctypes.c_void_p) for n in ('A', 'D', 'delta_bias', 'entering', 'lengths')]
+
+
+class ScanGradients(ctypes.Structure):
+    """``ovl_ssm_scan_gradients``"""
+    _fields_ = [('d_y', Sequence)] + [(n, ctypes.c_void_p) for n in
+                                      ('d_last', 'd_u', 'd_delta', 'd_z', 'd_B', 'd_C', 'd_A', 'd_D', 'd_delta_bias',
+                                       'd_entering')]
+
+
+class Conv(ctypes.Structure):
+    """``ovl_ssm_conv``"""
+    _fields_ = [(n, ctypes.c_uint32) for n in ('batch', 'length', 'channels', 'width')] + \
+               [('dtype', ctypes.c_int32), ('silu', ctypes.c_int32), ('x', Sequence), ('weight', ctypes.c_void_p),
+                ('bias', ctypes.c_void_p), ('kept', Sequence), ('lengths', ctypes.c_void_p)]
+
+
+_lib = None
+
+
+def library():
+    """The loaded library (loads it on first use); there is no fallback when it has not been built."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    if not os.path.exists(library_path):
+        raise RuntimeError('The state space library ' + library_path + ' has not been built. '
+                           'Run "python -m opveclib_amd.build" first.')
+    lib = ctypes.CDLL(library_path)
+    p, u64 = ctypes.c_void_p, ctypes.c_uint64
+    lib.ovl_ssm_scan_workspace_bytes.argtypes = [p, ctypes.c_int32]
+    lib.ovl_ssm_scan_saved_bytes.argtypes = [p]
+    lib.ovl_ssm_scan_forward.argtypes = [p, p, p, p, p, u64, p]
+    lib.ovl_ssm_scan_backward.argtypes = [p, p, p, p, u64, p]
+    lib.ovl_ssm_scan_step.argtypes = [p, p, ctypes.c_int64, p, p]
+    lib.ovl_ssm_conv_forward.argtypes = [p, p, p, p]
+    lib.ovl_ssm_conv_workspace_bytes.argtypes = [p]
+    lib.ovl_ssm_conv_backward.argtypes = [p, p, p, p, p, p, p, p, u64, p]
+    lib.ovl_ssm_conv_step.argtypes = [p, p, p]
+    for name in EXPORTED_SYMBOLS:
+        getattr(lib, name).restype = u64 if name.endswith('_bytes') else ctypes.c_int
+    lib.ovl_ssm_last_error.restype = ctypes.c_char_p
+    _lib = lib
+    return lib
+
+
+class StateSpaceError(RuntimeError):
+    def __init__(self, code, detail):
+        RuntimeError.__init__(self, 'ovl_ssm error %d: %s' % (code, detail))
+        self.code = code
+
+
+def _call(code):
+    if code != 0:
+        raise StateSpaceError(code, library().ovl_ssm_last_error().decode('utf-8', 'replace'))
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# arguments
+# ----------------------------------------------------------------------------------------------------------------------
+_codes = {}
+
+
+def _type_code(dtype):
+    """The element type's code; only these three types have kernels."""
+    if not _codes:
+        import torch
+        _codes.update({torch.float16: 1, torch.float32: 2, torch.bfloat16: 32})
+    code = _codes.get(dtype)
+    if code is None:
+        raise TypeError('sequences must be float32, float16 or bfloat16, got ' + str(dtype))
+    return code
+
+
+class _Arguments(object):
+    """Checks tensors of one call against its first one, and keeps those it had to copy alive until the launch."""
+
+    def __init__(self, torch, first, name):
+        self.torch = torch
+        if not isinstance(first, torch.Tensor):
+            raise TypeError(name + ' must be a torch tensor')
+        if first.device.type != 'cuda':
+            raise RuntimeError('the state space kernels run on an AMD GPU: tensors must live on a HIP device')
+        self.device = first.device
+        self.dtype = first.dtype
+        self.code = _type_code(first.dtype)
+        self.kept = []
+
+    def tensor(self, t, name, shape, dtype):
+        if not isinstance(t, self.torch.Tensor):
+            raise TypeError(name + ' must be a torch tensor')
+        if t.device != self.device:
+            raise TypeError('%s is on %s, expected %s' % (name, t.device, self.device))
+        if t.dtype != dtype:
+            raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
+        if tuple(t.shape) != shape:
+            raise TypeError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
+        return t
+
+    def side_by_side(self, t):
+        if t.stride(-1) != 1 and t.shape[-1] != 1:
+            t = t.contiguous()
+            self.kept.append(t)
+        return t
+
+    def sequence(self, t, name, shape):
+        """[batch, length, channels], or [batch, channels] for one token."""
+        if t is None:
+            return (None, 0, 0)
+        t = self.side_by_side(self.tensor(t, name, shape, self.dtype))
+        strides = t.stride()
+        return (t.data_ptr(), strides[0], strides[1] if len(shape) == 3 else 0)
+
+    def vectors(self, t, name, shape):
+        """[batch, length, groups, state], or without the length for one token; without the groups if there is one."""
+        t = self.side_by_side(self.tensor(t, name, shape, self.dtype))
+        strides = t.stride()
+        return (t.data_ptr(),) + strides[:-1]
+
+    def parameter(self, t, name, shape):
+        """A dense float32 tensor's address, or None."""
+        if t is None:
+            return None
+        t = self.tensor(t, name, shape, self.torch.float32)
+        if not t.is_contiguous():
+            t = t.contiguous()
+            self.kept.append(t)
+        return t.data_ptr()
+
+    def weights(self, t, name, shape):
+        """A parameter of the convolution: float32, or the sequences' type, which is converted."""
+        if t is None:
+            return None
+        if not isinstance(t, self.torch.Tensor):
+            raise TypeError(name + ' must be a torch tensor')
+        if t.dtype == self.dtype and t.dtype != self.torch.float32:
+            t = t.detach().float()
+            self.kept.append(t)
+        return self.parameter(t, name, shape)
+
+    def lengths(self, t, batch):
+        if t is None:
+            return None
+        t = self.tensor(t, 'lengths', (batch,), self.torch.int32)
+        if not t.is_contiguous():
+            t = t.contiguous()
+            self.kept.append(t)
+        return t.data_ptr()
+
+    def scratch(self, nbytes):
+        """Uninitialised device memory of that size: its address, or None for nothing."""
+        if nbytes == 0:
+            return None
+        t = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
+        self.kept.append(t)
+        return t.data_ptr()
+
+    def stream(self):
+        return self.torch.cuda.current_stream(self.device).cuda_stream
+
+
+def _on(torch, device):
+    """The device of the call as the current one; without the cost of switching where it is already."""
+    import contextlib
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# the scan
+# ----------------------------------------------------------------------------------------------------------------------
+def _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, token=False):
+    args = _Arguments(torch, u, 'u')
+    shape = tuple(u.shape)
+    if len(shape) != (2 if token else 3):
+        raise TypeError('u must be %s, got %s' % ('[batch, channels]' if token else '[batch, length, channels]', list(shape)))
+    batch, channels = shape[0], shape[-1]
+    length = 1 if token else shape[1]
+    if channels == 0:
+        raise TypeError('u must have at least one channel')
+    if not isinstance(A, torch.Tensor) or A.dim() != 2 or A.shape[0] != channels:
+        raise TypeError('A must be [channels, state] with %d channels' % channels)
+    n = A.shape[1]
+    if not 1 <= n <= MAX_STATE:
+        raise TypeError('A must have 1 to %d state entries per channel, got %d' % (MAX_STATE, n))
+    groups = 1
+    if not isinstance(B, torch.Tensor):
+        raise TypeError('B must be a torch tensor')
+    lead = shape[:-1]
+    if B.dim() == len(lead) + 2:
+        groups = B.shape[-2]
+        if groups < 1 or channels % groups != 0:
+            raise TypeError('the groups of B and C must divide the %d channels, got %d' % (channels, groups))
+        vector_shape = lead + (groups, n)
+    else:
+        vector_shape = lead + (n,)
+    b = args.vectors(B, 'B', vector_shape)
+    c = args.vectors(C, 'C', vector_shape)
+
+    def four(v):
+        v = list(v)
+        if token:
+            v.insert(2, 0)
+        return tuple(v) if len(v) == 4 else tuple(v) + (0,)
+
+    scan = Scan(batch, length, channels, n, groups, args.code, 1 if softplus else 0,
+                args.sequence(u, 'u', shape), args.sequence(delta, 'delta', shape), args.sequence(z, 'z', shape),
+                four(b), four(c),
+                args.parameter(A, 'A', (channels, n)), args.parameter(D, 'D', (channels,)),
+                args.parameter(delta_bias, 'delta_bias', (channels,)),
+                None if token else args.parameter(state, 'state', (batch, channels, n)),
+                args.lengths(lengths, batch))
+    return args, scan, vector_shape
+
+
+def _scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, keep):
+    import torch
+    args, scan, _ = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths)
+    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    last = torch.empty((scan.batch, scan.channels, scan.state), dtype=torch.float32, device=u.device)
+    if y.numel() == 0:
+        return y, (last.zero_() if state is None else last.copy_(state.detach())), None
+    lib = library()
+    ref = ctypes.byref(scan)
+    saved = None
+    if keep:
+        saved = torch.empty(lib.ovl_ssm_scan_saved_bytes(ref) // 4, dtype=torch.float32, device=u.device)
+    need = lib.ovl_ssm_scan_workspace_bytes(ref, 0)
+    with _on(torch, args.device):
+        _call(lib.ovl_ssm_scan_forward(ref, y.data_ptr(), last.data_ptr(), None if saved is None else saved.data_ptr(),
+                                       args.scratch(need), need, args.stream()))
+    return y, last, saved
+
+
+def scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False, state=None, lengths=None):
+    """
+    The selective state space scan: for every channel c, state entry n and token t
+
+        dt = delta[t, c] + delta_bias[c], with ``softplus`` log(1 + exp(.)) of it
+        h[t, n] = exp(dt * A[c, n]) * h[t - 1, n] + dt * u[t, c] * B[t, n]
+        y[t, c] = sum over n of C[t, n] * h[t, n] + D[c] * u[t, c], times z[t, c] * sigmoid(z[t, c]) with a gate ``z``
+
+    :param u, delta, z: [batch, length, channels]
+    :param A: [channels, state], float32, up to 64 state entries
+    :param B, C: [batch, length, state], or [batch, length, groups, state]: neighbouring channels / groups channels share
+        the vectors of their group
+    :param D, delta_bias: [channels], float32
+    :param state: [batch, channels, state], float32: the state before the first token; zero if not given
+    :return: (y [batch, length, channels], the state after the last token)
+    """
+    return _scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, False)[:2]
+
+
+def scan_grad(u, delta, A, B, C, d_y, D=None, z=None, delta_bias=None, softplus=False, state=None, lengths=None,
+              d_last=None, saved=None):
+    """
+    Gradients of :func:`scan` given those of its outputs (``d_last`` may be left out).  The states inside the sequence are
+    recomputed unless ``saved`` holds those that :func:`scan_torch` keeps.
+
+    :return: (d_u, d_delta, d_A, d_B, d_C, d_D, d_z, d_delta_bias, d_state), None for what was not given
+    """
+    import torch
+    args, scan_, vector_shape = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths)
+
+    def new(shape, dtype, wanted=True):
+        return torch.empty(shape, dtype=dtype, device=u.device) if wanted else None
+
+    f32 = torch.float32
+    state_shape = (scan_.batch, scan_.channels, scan_.state)
+    d_y_at = args.sequence(d_y, 'd_y', tuple(u.shape))
+    if d_y_at[0] is None:
+        raise TypeError('d_y must be a torch tensor')
+    out = (new(u.shape, u.dtype), new(u.shape, u.dtype), new(A.shape, f32), new(vector_shape, u.dtype),
+           new(vector_shape, u.dtype), new((scan_.channels,), f32, D is not None), new(u.shape, u.dtype, z is not None),
+           new((scan_.channels,), f32, delta_bias is not None), new(state_shape, f32, state is not None))
+    if u.numel() == 0:
+        for t in out:
+            if t is not None:
+                t.zero_()
+        if out[8] is not None and d_last is not None:
+            out[8].copy_(args.tensor(d_last, 'd_last', state_shape, f32).detach())
+        return out
+    d_last_at = args.parameter(d_last, 'd_last', state_shape)
+    at = [None if t is None else t.data_ptr() for t in out]
+    gradients = ScanGradients(d_y_at, d_last_at, at[0], at[1], at[6], at[3], at[4], at[2], at[5], at[7], at[8])
+    lib = library()
+    ref = ctypes.byref(scan_)
+    with _on(torch, args.device):
+        stream = args.stream()
+        need = lib.ovl_ssm_scan_saved_bytes(ref)
+        if saved is None:
+            saved = torch.empty(need // 4, dtype=f32, device=u.device)
+            work = lib.ovl_ssm_scan_workspace_bytes(ref, 0)
+            _call(lib.ovl_ssm_scan_forward(ref, None, None, saved.data_ptr(), args.scratch(work), work, stream))
+        else:
+            args.tensor(saved, 'saved', (need // 4,), f32)
+            if not saved.is_contiguous():
+                raise TypeError('saved must be contiguous')
+        work = lib.ovl_ssm_scan_workspace_bytes(ref, 1)
+        _call(lib.ovl_ssm_scan_backward(ref, saved.data_ptr(), ctypes.byref(gradients), args.scratch(work), work, stream))
+    return out
+
+
+def scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False):
+    """
+    :func:`scan` for one new token per sequence: ``u``, ``delta``, ``z`` are [batch, channels], ``B`` and ``C`` [batch,
+    state] or [batch, groups, state].  ``state`` [batch, channels, state], float32, is updated in place; it may be a part
+    of a larger buffer along its first axis (its other axes are dense, and its sequences do not overlap).
+
+    :return: y [batch, channels]
+    """
+    import torch
+    args, scan_, _ = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, None, None, token=True)
+    shape = (scan_.batch, scan_.channels, scan_.state)
+    stride = _in_place(args, state, shape, torch.float32)[0]
+    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    if y.numel() == 0:
+        return y
+    with _on(torch, args.device):
+        _call(library().ovl_ssm_scan_step(ctypes.byref(scan_), state.data_ptr(), stride, y.data_ptr(), args.stream()))
+    return y
+
+
+def _in_place(args, state, shape, dtype):
+    """Strides of a [batch, .., ..] tensor that is overwritten: dense but for the first axis, whose parts lie apart."""
+    args.tensor(state, 'state', shape, dtype)
+    if state.requires_grad and args.torch.is_grad_enabled():
+        raise TypeError('state is overwritten and must not require a gradient')
+    strides = state.stride()
+    inner = shape[1] * shape[2]
+    if inner > 0 and not ((shape[2] == 1 or strides[2] == 1) and (shape[1] == 1 or strides[1] == shape[2])
+                          and (shape[0] <= 1 or strides[0] >= inner)):
+        raise TypeError('state is overwritten: its sequences must be dense and apart, got strides ' + str(strides))
+    return strides[0], shape[2]
+
+
+_functions = {}
+
+
+def _differentiable(name):
+    """The autograd functions, made on first use (torch is imported late)."""
+    if _functions:
+        return _functions[name]
+    import torch
+    once = torch.autograd.function.once_differentiable
+
+    class _Scan(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, u, delta, A, B, C, D, z, delta_bias, state, lengths, softplus):
+            y, last, saved = _scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths,
+                                   any(ctx.needs_input_grad))
+            ctx.softplus = softplus
+            ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, state, lengths, saved)
+            return y, last
+
+        @staticmethod
+        @once
+        def backward(ctx, d_y, d_last):
+            u, delta, A, B, C, D, z, delta_bias, state, lengths, saved = ctx.saved_tensors
+            grads = scan_grad(u, delta, A, B, C, d_y, D, z, delta_bias, ctx.softplus, state, lengths, d_last, saved)
+            return grads + (None, None)
+
+    class _Conv(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias, state, lengths, activation):
+            ctx.activation = activation
+            ctx.save_for_backward(x, weight, bias, state, lengths)
+            return conv(x, weight, bias, activation, state, lengths)
+
+        @staticmethod
+        @once
+        def backward(ctx, d_y, d_last):
+            x, weight, bias, state, lengths = ctx.saved_tensors
+            grads = conv_grad(x, weight, d_y, bias, ctx.activation, state, lengths, d_last)
+            return grads + (None, None)
+
+    _functions.update(scan=_Scan, conv=_Conv)
+    return _functions[name]
+
+
+def scan_torch(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False, state=None, lengths=None):
+    """:func:`scan` as a differentiable PyTorch function.  Where a gradient is wanted the forward pass keeps the state
+    before every 16th token (4 * state / 16 bytes for each element of ``u``) for the backward pass."""
+    return _differentiable('scan').apply(u, delta, A, B, C, D, z, delta_bias, state, lengths, softplus)
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# the short causal convolution
+# ----------------------------------------------------------------------------------------------------------------------
+def _silu(activation):
+    if activation not in (None, 'silu'):
+        raise ValueError("activation must be None or 'silu', got " + repr(activation))
+    return 0 if activation is None else 1
+
+
+def _describe_conv(torch, x, weight, bias, activation, state, lengths, token=False):
+    args = _Arguments(torch, x, 'x')
+    shape = tuple(x.shape)
+    if len(shape) != (2 if token else 3):
+        raise TypeError('x must be %s, got %s' % ('[batch, channels]' if token else '[batch, length, channels]', list(shape)))
+    batch, channels = shape[0], shape[-1]
+    if channels == 0:
+        raise TypeError('x must have at least one channel')
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] != channels:
+        raise TypeError('weight must be [channels, width] with %d channels' % channels)
+    width = weight.shape[1]
+    if not 1 <= width <= MAX_WIDTH:
+        raise TypeError('weight must have 1 to %d taps per channel, got %d' % (MAX_WIDTH, width))
+    kept_shape = (batch, width - 1, channels)
+    if token:
+        strides = _in_place(args, state, kept_shape, x.dtype)
+        kept = (state.data_ptr() if width > 1 else None, strides[0], strides[1])
+    elif state is None or width == 1:
+        if state is not None:
+            args.tensor(state, 'state', kept_shape, x.dtype)
+        kept = (None, 0, 0)
+    else:
+        kept = args.sequence(state, 'state', kept_shape)
+    conv_ = Conv(batch, 1 if token else shape[1], channels, width, args.code, _silu(activation),
+                 args.sequence(x, 'x', shape), args.weights(weight, 'weight', (channels, width)),
+                 args.weights(bias, 'bias', (channels,)), kept, args.lengths(lengths, batch))
+    return args, conv_, kept_shape
+
+
+def conv(x, weight, bias=None, activation=None, state=None, lengths=None):
+    """
+    Causal convolution of every channel with its own few taps: with ``line`` the ``width - 1`` tokens of ``state`` (zeros
+    if not given) followed by ``x``,
+
+        y[t, c] = bias[c] + sum over k of weight[c, k] * line[t + k, c], times its own sigmoid with activation 'silu'
+
+    :param x: [batch, length, channels]
+    :param weight: [channels, width], width 1 to 4; bias: [channels]; both float32 or of the type of ``x``
+    :param state: [batch, width - 1, channels] of the type of ``x``: the tokens before the first
+    :return: (y [batch, length, channels], the last width - 1 tokens, which a later call takes as ``state``)
+    """
+    import torch
+    args, conv_, kept_shape = _describe_conv(torch, x, weight, bias, activation, state, lengths)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    last = torch.empty(kept_shape, dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y, (last.zero_() if state is None else last.copy_(state.detach()))
+    with _on(torch, args.device):
+        _call(library().ovl_ssm_conv_forward(ctypes.byref(conv_), y.data_ptr(), last.data_ptr(), args.stream()))
+    return y, last
+
+
+def conv_grad(x, weight, d_y, bias=None, activation=None, state=None, lengths=None, d_last=None):
+    """
+    Gradients of :func:`conv` given those of its outputs (``d_last`` may be left out); the convolution is recomputed.
+
+    :return: (d_x, d_weight, d_bias, d_state), None for what was not given; d_weight and d_bias in their tensors' types
+    """
+    import torch
+    args, conv_, kept_shape = _describe_conv(torch, x, weight, bias, activation, state, lengths)
+    f32 = torch.float32
+    d_y_at = args.sequence(d_y, 'd_y', tuple(x.shape))
+    if d_y_at[0] is None:
+        raise TypeError('d_y must be a torch tensor')
+    d_last_at = args.sequence(d_last, 'd_last', kept_shape)
+    d_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    d_weight = torch.empty(tuple(weight.shape), dtype=f32, device=x.device)
+    d_bias = None if bias is None else torch.empty((conv_.channels,), dtype=f32, device=x.device)
+    d_state = None if state is None else torch.empty(kept_shape, dtype=x.dtype, device=x.device)
+    if x.numel() == 0:
+        d_weight.zero_()
+        if d_bias is not None:
+            d_bias.zero_()
+        if d_state is not None:
+            d_state.zero_() if d_last is None else d_state.copy_(d_last.detach())
+    else:
+        lib = library()
+        ref = ctypes.byref(conv_)
+        need = lib.ovl_ssm_conv_workspace_bytes(ref)
+        d_y_seq, d_last_seq = Sequence(*d_y_at), Sequence(*d_last_at)
+        with _on(torch, args.device):
+            _call(lib.ovl_ssm_conv_backward(ref, ctypes.byref(d_y_seq),
+                                            None if d_last_at[0] is None else ctypes.byref(d_last_seq), d_x.data_ptr(),
+                                            None if d_state is None or conv_.width == 1 else d_state.data_ptr(),
+                                            d_weight.data_ptr(), None if d_bias is None else d_bias.data_ptr(),
+                                            args.scratch(need), need, args.stream()))
+    return (d_x, d_weight.to(weight.dtype), None if d_bias is None else d_bias.to(bias.dtype), d_state)
+
+
+def conv_step(x, state, weight, bias=None, activation=None):
+    """
+    :func:`conv` for one new token per sequence: ``x`` is [batch, channels]; ``state`` [batch, width - 1, channels] is
+    updated in place; it may be a part of a larger buffer along its first axis (its other axes are dense, and its
+    sequences do not overlap).
+
+    :return: y [batch, channels]
+    """
+    import torch
+    args, conv_, _ = _describe_conv(torch, x, weight, bias, activation, state, None, token=True)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    with _on(torch, args.device):
+        _call(library().ovl_ssm_conv_step(ctypes.byref(conv_), y.data_ptr(), args.stream()))
+    return y
+
+
+def conv_torch(x, weight, bias=None, activation=None, state=None, lengths=None):
+    """:func:`conv` as a differentiable PyTorch function (gradients through :func:`conv_grad`)."""
+    return _differentiable('conv').apply(x, weight, bias, state, lengths, activation)

@@ -1,0 +1,177 @@
+"""The state space and norm libraries without a GPU: headers and bindings agree, and bad arguments are refused, by the C
+entry points before any GPU work and by the Python functions with the errors the other hand-written kernels use."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+from opveclib_amd import rms_norm, state_space
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+EINVAL = 6
+
+
+def declared_functions(header):
+    text = open(os.path.join(ROOT, 'include', header)).read()
+    text = re.sub(r'/\*.*?\*/', '', text, flags=re.S)
+    return sorted(set(re.findall(r'\b(ovl_[a-z_0-9]+)\s*\(', text)))
+
+
+@pytest.fixture(scope='module')
+def libraries():
+    for module in (state_space, rms_norm):
+        if not os.path.exists(module.library_path):
+            module.build()
+    return state_space.library(), rms_norm.library()
+
+
+def test_headers_and_bindings_agree(libraries):
+    for header, module in (('ovl_ssm.h', state_space), ('ovl_norm.h', rms_norm)):
+        assert declared_functions(header) == sorted(module.EXPORTED_SYMBOLS)
+        raw = ctypes.CDLL(module.library_path)
+        for name in declared_functions(header):
+            assert hasattr(raw, name), name
+
+
+def test_missing_libraries_are_loud_errors(monkeypatch):
+    for module in (state_space, rms_norm):
+        monkeypatch.setattr(module, '_lib', None)
+        monkeypatch.setattr(module, 'library_path', '/nonexistent/lib.so')
+        with pytest.raises(RuntimeError):
+            module.library()
+
+
+# addresses that no refused call looks at
+P = 4096
+
+
+def scan_struct(**changes):
+    sequence = state_space.Sequence(P, 64, 8)
+    vectors = state_space.Vectors(P, 64, 4, 4)
+    s = state_space.Scan(2, 8, 8, 4, 1, 2, 1, sequence, sequence, state_space.Sequence(), vectors, vectors, P, P, P, None, None)
+    for name, value in changes.items():
+        setattr(s, name, value)
+    return s
+
+
+def test_scan_entry_points_refuse(libraries):
+    lib, _ = libraries
+    empty = state_space.Sequence()
+    for changes, word in (({'batch': 0}, b'positive'), ({'length': 0}, b'positive'), ({'channels': 0}, b'positive'),
+                          ({'state': 0}, b'positive'), ({'groups': 0}, b'positive'), ({'state': 65}, b'64 state'),
+                          ({'groups': 3}, b'divide'), ({'dtype': 3}, b'element type'), ({'u': empty}, b'null'),
+                          ({'delta': empty}, b'null'), ({'B': state_space.Vectors()}, b'null'),
+                          ({'C': state_space.Vectors()}, b'null'), ({'A': None}, b'null'),
+                          ({'length': (1 << 30) + 1}, b'2^30'), ({'batch': 1 << 30, 'channels': 1 << 20}, b'too many')):
+        s = scan_struct(**changes)
+        ref = ctypes.byref(s)
+        assert lib.ovl_ssm_scan_forward(ref, P, P, None, None, 0, None) == EINVAL, changes
+        assert word in lib.ovl_ssm_last_error(), changes
+        assert lib.ovl_ssm_scan_backward(ref, P, ctypes.byref(state_space.ScanGradients()), P, 1 << 40, None) == EINVAL
+        assert lib.ovl_ssm_scan_workspace_bytes(ref, 0) == 0 and lib.ovl_ssm_scan_saved_bytes(ref) == 0
+    s = scan_struct()
+    ref = ctypes.byref(s)
+    assert lib.ovl_ssm_scan_forward(None, P, P, None, None, 0, None) == EINVAL
+    assert lib.ovl_ssm_scan_forward(ref, P, None, None, None, 0, None) == EINVAL
+    assert lib.ovl_ssm_scan_forward(ref, None, None, None, None, 0, None) == EINVAL
+    assert lib.ovl_ssm_scan_backward(ref, None, ctypes.byref(state_space.ScanGradients()), P, 1 << 40, None) == EINVAL
+    assert lib.ovl_ssm_scan_backward(ref, P, ctypes.byref(state_space.ScanGradients()), P, 1 << 40, None) == EINVAL
+    gradients = state_space.ScanGradients(state_space.Sequence(P, 64, 8), None, *([P] * 9))
+    need = lib.ovl_ssm_scan_workspace_bytes(ref, 1)
+    assert need > 0
+    for workspace, size in ((None, need), (P, need - 1), (P + 4, need)):
+        assert lib.ovl_ssm_scan_backward(ref, P, ctypes.byref(gradients), workspace, size, None) == EINVAL
+        assert b'workspace' in lib.ovl_ssm_last_error()
+    assert lib.ovl_ssm_scan_step(ref, P, 32, P, None) == EINVAL             # eight tokens are no step
+    s.length = 1
+    assert lib.ovl_ssm_scan_step(ref, None, 32, P, None) == EINVAL
+    s.lengths = P
+    assert lib.ovl_ssm_scan_step(ref, P, 32, P, None) == EINVAL
+    long = scan_struct(batch=1, length=1 << 14)                             # split into chunks: needs scratch memory
+    need = lib.ovl_ssm_scan_workspace_bytes(ctypes.byref(long), 0)
+    assert need > 0
+    assert lib.ovl_ssm_scan_forward(ctypes.byref(long), P, P, None, P, need - 1, None) == EINVAL
+
+
+def test_conv_entry_points_refuse(libraries):
+    lib, _ = libraries
+    sequence = state_space.Sequence(P, 64, 8)
+
+    def struct(**changes):
+        s = state_space.Conv(2, 8, 8, 4, 2, 1, sequence, P, P, sequence, None)
+        for name, value in changes.items():
+            setattr(s, name, value)
+        return s
+
+    for changes in ({'batch': 0}, {'length': 0}, {'channels': 0}, {'width': 0}, {'width': 5}, {'dtype': 9},
+                    {'x': state_space.Sequence()}, {'weight': None}, {'length': (1 << 30) + 1},
+                    {'batch': 1 << 31, 'channels': 1 << 31}):
+        ref = ctypes.byref(struct(**changes))
+        assert lib.ovl_ssm_conv_forward(ref, P, P, None) == EINVAL, changes
+        assert lib.ovl_ssm_conv_workspace_bytes(ref) == 0
+        assert lib.ovl_ssm_conv_backward(ref, ctypes.byref(sequence), None, P, P, P, P, P, 1 << 40, None) == EINVAL
+    s = struct()
+    ref = ctypes.byref(s)
+    assert lib.ovl_ssm_conv_forward(ref, None, P, None) == EINVAL
+    assert lib.ovl_ssm_conv_forward(ref, P, None, None) == EINVAL
+    need = lib.ovl_ssm_conv_workspace_bytes(ref)
+    assert need > 0
+    assert lib.ovl_ssm_conv_backward(ref, ctypes.byref(sequence), None, P, P, P, P, P, need - 1, None) == EINVAL
+    assert lib.ovl_ssm_conv_backward(ref, None, None, P, P, P, P, P, need, None) == EINVAL
+    assert lib.ovl_ssm_conv_step(ref, P, None) == EINVAL
+    one = struct(length=1, kept=state_space.Sequence())
+    assert lib.ovl_ssm_conv_step(ctypes.byref(one), P, None) == EINVAL
+
+
+def test_norm_entry_points_refuse(libraries):
+    _, lib = libraries
+
+    def struct(**changes):
+        s = rms_norm.Norm(4, 16, 32, 32, 2, 1e-5, P, 16, None, 0, P)
+        for name, value in changes.items():
+            setattr(s, name, value)
+        return s
+
+    for changes in ({'rows': 0}, {'columns': 0}, {'columns': 32769}, {'dtype': 3}, {'residual_dtype': 1}, {'weight_dtype': 1},
+                    {'x': None}, {'weight': None}):
+        ref = ctypes.byref(struct(**changes))
+        assert lib.ovl_norm_forward(ref, P, P, None) == EINVAL, changes
+        assert lib.ovl_norm_forward_quantized(ref, 0, P, P, P, None) == EINVAL, changes
+        assert lib.ovl_norm_backward(ref, P, 16, None, 0, P, P, P, P, 1 << 40, None) == EINVAL, changes
+        assert lib.ovl_norm_workspace_bytes(ref) == 0
+    s = struct()
+    ref = ctypes.byref(s)
+    assert lib.ovl_norm_forward(None, P, P, None) == EINVAL
+    assert lib.ovl_norm_forward(ref, None, None, None) == EINVAL
+    assert lib.ovl_norm_forward_quantized(ref, 64, P, P, None, None) == EINVAL
+    assert b'128' in lib.ovl_norm_last_error()
+    assert lib.ovl_norm_forward_quantized(ref, 0, P, None, None, None) == EINVAL
+    need = lib.ovl_norm_workspace_bytes(ref)
+    assert lib.ovl_norm_backward(ref, P, 16, None, 0, P, P, P, P, need - 1, None) == EINVAL
+    assert lib.ovl_norm_backward(ref, P, 16, None, 0, P, P, None, P, need, None) == EINVAL
+    s.residual = P
+    assert lib.ovl_norm_forward(ref, P, None, None) == EINVAL
+
+
+def test_python_functions_refuse_host_tensors_and_other_things():
+    u = torch.zeros(2, 4, 8)
+    A = torch.zeros(8, 4)
+    B = torch.zeros(2, 4, 4)
+    with pytest.raises(RuntimeError):
+        state_space.scan(u, u, A, B, B)
+    with pytest.raises(RuntimeError):
+        state_space.scan_step(torch.zeros(2, 8, 4), u[:, 0], u[:, 0], A, B[:, 0], B[:, 0])
+    with pytest.raises(RuntimeError):
+        state_space.conv(u, torch.zeros(8, 4))
+    with pytest.raises(RuntimeError):
+        rms_norm.rms_norm(u, torch.ones(8))
+    for call in (lambda: state_space.scan(u.numpy(), u, A, B, B), lambda: state_space.conv(None, A),
+                 lambda: rms_norm.rms_norm([1.0], A)):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(ValueError):
+        state_space._silu('relu')
+    with pytest.raises(ValueError):
+        rms_norm.rms_norm_quantized(u, torch.ones(8), group=64)
