@@ -20,7 +20,8 @@
  * after its last token, outputs and gradients behind it are zero, and what the inputs hold there is not looked at.
  *
  * Conventions: tensor memory belongs to the caller and must be device accessible; sequences have their channels side by
- * side, batch and token strides (in elements) are free; outputs are dense.  All sums, states and gradients of
+ * side, batch and token strides (in elements) are free, but for the scan's token strides, which are 0 to 2^25; outputs are
+ * dense.  All sums, states and gradients of
  * parameters are float32; only what is stored in the tensors' type is rounded, once.  The functions enqueue kernels on
  * `hip_stream`, return without synchronising, allocate nothing (scratch memory is handed in, its size is asked for
  * first) and give the same bits for the same call.  They return an ovl_status (ovl_launch.h): OVL_EINVAL for arguments
@@ -37,6 +38,9 @@ extern "C" {
 
 /* Element types of the sequences: the codes of ovl_launch.h, and bfloat16, which the operator IR does not have. */
 enum ovl_ssm_dtype { OVL_SSM_FLOAT16 = 1, OVL_SSM_FLOAT32 = 2, OVL_SSM_BFLOAT16 = 32 };
+
+/* Largest distance of two tokens of a sequence, in elements, that the scan takes. */
+#define OVL_SSM_MAX_TOKEN_STRIDE (1 << 25)
 
 /* One sequence tensor [batch, length, channels], channels side by side; data NULL: absent. */
 typedef struct ovl_ssm_sequence {

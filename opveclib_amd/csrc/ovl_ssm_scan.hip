@@ -36,7 +36,9 @@ constexpr uint32_t TILE = 16;               // tokens per tile; states are kept 
 constexpr uint32_t QUADS = TILE / 4;        // groups of four tokens
 constexpr uint32_t WAVES = 4;
 constexpr uint32_t THREADS = 64 * WAVES;
-constexpr uint32_t BLOCK = 16 * WAVES;      // channels of a workgroup
+constexpr uint32_t BLOCK = 64;              // channels of a workgroup
+constexpr uint32_t STEP = 8;                // tokens that a lane with a channel of its own takes at a time
+constexpr int RESIDENT = 2;                 // wavefronts of the kernels with a channel per lane on a SIMD
 
 constexpr float LOG2E = 0x1.715476p+0f, LN2 = 0x1.62e43p-1f;
 
@@ -57,24 +59,25 @@ template <typename T> struct scan_args {
 // Where a workgroup works: sequence, group, block of channels, chunk.
 struct place {
     uint32_t b, g, block, chunk;
-    uint32_t q, channel;                    // lane of the quad; channel (clamped to a valid one)
+    uint32_t q, channel;                    // lane of its channel's team; channel (clamped to a valid one)
     bool active;                            // whether the channel is one of the group's
     uint32_t first, last;                   // tiles
     uint32_t end;                           // first token behind the sequence
 };
 
-template <typename T>
-__device__ __forceinline__ place find_place(const scan_args<T>& p, uint32_t chunk_base, uint32_t chunks) {
+// TEAM: lanes per channel.  `unit` counts blocks of channels first, so that neighbouring units read the same B and C.
+template <uint32_t TEAM, typename T>
+__device__ __forceinline__ place find_place(const scan_args<T>& p, uint32_t unit, uint32_t lane, uint32_t chunk_base, uint32_t chunks) {
     place w;
-    uint32_t id = blockIdx.x;
-    w.chunk = chunk_base + id % chunks;
-    id /= chunks;
+    uint32_t id = unit;
     w.block = id % p.blocks;
     id /= p.blocks;
     w.g = id % p.groups;
-    w.b = id / p.groups;
-    w.q = threadIdx.x & 3u;
-    uint32_t c = w.block * BLOCK + threadIdx.x / 4u;
+    id /= p.groups;
+    w.chunk = chunk_base + id % chunks;
+    w.b = id / chunks;
+    w.q = lane % TEAM;
+    uint32_t c = w.block * BLOCK + lane / TEAM;
     w.active = c < p.per_group;
     c = w.active ? c : p.per_group - 1u;
     w.channel = w.g * p.per_group + c;
@@ -98,56 +101,162 @@ __device__ __forceinline__ float softplus_(float x) {
     float e = ovl_lane::exp2_(p);
     e = ax < 100.0f ? fmaf(e * LN2, low, e) : e;
     const float w = 1.0f + e;
-    const float lost = e - (w - 1.0f);
-    const float log1p = fmaf(lost, ovl_lane::rcp_(w), ovl_lane::log2_(w) * LN2);
-    return fmaxf(x, 0.0f) + log1p;
+    const float lost = e - (w - 1.0f);      // to be divided by w; it matters only where w is nearly one
+    const float log1p = fmaf(ovl_lane::log2_(w), LN2, lost);
+    return ovl_lane::positive(x) + log1p;
 }
 
 __device__ __forceinline__ float sigmoid_(float x) { return ovl_lane::rcp_(1.0f + ovl_lane::exp2_(-x * LOG2E)); }
 
-// Every lane's raw elements of the four groups of tokens of a tile: token t0 + 4 j + q.  Tokens behind the length are
-// read as the last one (the values are not used).
-template <typename T>
-__device__ __forceinline__ void load_tile(T (&to)[QUADS], const sequence<T>& s, const place& w, uint32_t t0, uint32_t length) {
-    const T* base = s.data + (int64_t)w.b * s.batch_stride + w.channel;
+// A sequence tensor as a lane reads it: N tokens of its channel, PACE tokens apart, of a tile of N * PACE tokens.  The
+// tile's address and the tokens' offsets are the same for the whole wavefront and stay in scalar registers; a lane adds 32
+// bits of its own (the host has checked that they suffice).  The offsets are made anew for every tile: kept, those of all
+// tensors would not fit the scalar registers, and their places in vector registers cost wavefronts.
+template <typename T, uint32_t N, uint32_t PACE> struct reader {
+    const T* tile;
+    uint32_t token_bytes, own;
+    __device__ __forceinline__ reader(const sequence<T>& s, const place& w, uint32_t t0)
+        : tile(s.data + (int64_t)w.b * s.batch_stride + (int64_t)t0 * s.token_stride),
+          token_bytes((uint32_t)s.token_stride * (uint32_t)sizeof(T)),
+          own(w.q * token_bytes + w.channel * (uint32_t)sizeof(T)) {}
+    __device__ __forceinline__ void load(T (&to)[N]) const {
+        const ovl_lane::region r(tile);
+        const uint32_t pace = ovl_lane::anew(token_bytes) * PACE;
 #pragma unroll
-    for (uint32_t j = 0; j < QUADS; ++j) to[j] = base[(int64_t)min(t0 + 4u * j + w.q, length - 1u) * s.token_stride];
-}
-
-// The elements of a tile of B or C that this thread takes to LDS, NP = 4 S entries per token.
-template <typename T, int S> struct vector_stage {
-    static constexpr uint32_t NP = 4 * S, ALL = TILE * NP, PER = (ALL + THREADS - 1) / THREADS;
-    T raw[PER];
-    __device__ __forceinline__ void load(const vectors<T>& v, const place& w, uint32_t t0, uint32_t length, uint32_t n) {
-        const T* base = v.data + (int64_t)w.b * v.batch_stride + (int64_t)w.g * v.group_stride;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) {
-            const uint32_t at = threadIdx.x + i * THREADS;
-            raw[i] = base[(int64_t)min(t0 + at / NP, length - 1u) * v.token_stride + min(at % NP, n - 1u)];
-        }
+        for (uint32_t j = 0; j < N; ++j) to[j] = r.template load<T>(own, j * pace);
     }
-    // Entries past the state and tokens behind the sequence become zero: they then add nothing anywhere.
-    __device__ __forceinline__ void store(float* lds, const place& w, uint32_t t0, uint32_t n) const {
+    // Only `left` tokens (at least one) are there: those behind are read as the last; the values are not used.
+    __device__ __forceinline__ void load_some(T (&to)[N], uint32_t left, uint32_t first) const {
+        const ovl_lane::region r(tile);
+        const uint32_t bytes = ovl_lane::anew(token_bytes);
 #pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) {
-            const uint32_t at = threadIdx.x + i * THREADS;
-            if (at < ALL) lds[at] = (at % NP < n && t0 + at / NP < w.end) ? widen<T>(raw[i]) : 0.0f;
-        }
+        for (uint32_t j = 0; j < N; ++j)
+            to[j] = r.template load<T>(own + (min(PACE * j + first, left - 1u) - first) * bytes, 0u);
+    }
+    // DIRECTION 1 or -1
+    template <int DIRECTION> __device__ __forceinline__ void move() {
+        const char* at = reinterpret_cast<const char*>(tile);
+        const uint64_t bytes = N * PACE * (uint64_t)token_bytes;
+        tile = reinterpret_cast<const T*>(DIRECTION > 0 ? at + bytes : at - bytes);
     }
 };
 
-template <int S> __device__ __forceinline__ void load_states(float (&h)[S], const float* from) {
+// Where a lane writes dense output sequences; several outputs of one shape share it.
+template <typename T, uint32_t N, uint32_t PACE> struct writer {
+    uint64_t tile;                          // in bytes
+    uint32_t token_bytes, own;
+    __device__ __forceinline__ writer(const place& w, uint32_t length, uint32_t channels, uint32_t t0)
+        : tile(((uint64_t)w.b * length + t0) * channels * sizeof(T)), token_bytes(channels * (uint32_t)sizeof(T)),
+          own(w.q * token_bytes + w.channel * (uint32_t)sizeof(T)) {}
+    __device__ __forceinline__ void store(T* to, const T (&x)[N]) const {
+        const ovl_lane::region r(reinterpret_cast<char*>(to) + tile);
+        const uint32_t pace = ovl_lane::anew(token_bytes) * PACE;
 #pragma unroll
-    for (int s = 0; s < S; ++s) h[s] = from[s];
+        for (uint32_t j = 0; j < N; ++j) r.template store<T>(x[j], own, j * pace);
+    }
+    // the first `left` tokens of the tile
+    __device__ __forceinline__ void store_some(T* to, const T (&x)[N], uint32_t left, uint32_t first) const {
+        const ovl_lane::region r(reinterpret_cast<char*>(to) + tile);
+        const uint32_t pace = ovl_lane::anew(token_bytes) * PACE;
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j)
+            if (PACE * j + first < left) r.template store<T>(x[j], own, j * pace);
+    }
+    template <int DIRECTION> __device__ __forceinline__ void move() { tile += DIRECTION * (int64_t)(N * PACE) * token_bytes; }
+};
+
+// The elements of a tile of B or C that this thread takes to LDS: TOKENS tokens of NP entries.
+template <typename T, uint32_t NP, uint32_t TOKENS, uint32_t LANES> struct vector_stage {
+    static constexpr uint32_t ALL = TOKENS * NP, PER = (ALL + LANES - 1) / LANES;
+    const T* tile;
+    uint32_t token_bytes, own[PER];
+    uint32_t lane;
+    T raw[PER];
+    __device__ __forceinline__ vector_stage(const vectors<T>& v, const place& w, uint32_t lane_, uint32_t t0, uint32_t n)
+        : tile(v.data + (int64_t)w.b * v.batch_stride + (int64_t)w.g * v.group_stride + (int64_t)t0 * v.token_stride),
+          token_bytes((uint32_t)v.token_stride * (uint32_t)sizeof(T)), lane(lane_) {
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint32_t at = (lane + i * LANES) % ALL;
+            own[i] = at / NP * token_bytes + min(at % NP, n - 1u) * (uint32_t)sizeof(T);
+        }
+    }
+    __device__ __forceinline__ void load() {
+        const ovl_lane::region r(tile);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) raw[i] = r.template load<T>(own[i], 0u);
+    }
+    __device__ __forceinline__ void load_some(uint32_t left) {
+        const ovl_lane::region r(tile);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint32_t token = (lane + i * LANES) % ALL / NP;
+            raw[i] = r.template load<T>(own[i] - (token < left ? 0u : (token - left + 1u) * token_bytes), 0u);
+        }
+    }
+    // Entries past the state and tokens behind the sequence (`tokens` of the tile's are in it) become zero: they then add
+    // nothing anywhere.
+    __device__ __forceinline__ void store(float* lds, uint32_t tokens, uint32_t n) const {
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint32_t at = lane + i * LANES;
+            if (ALL % LANES == 0u || at < ALL) lds[at] = (at % NP < n && at / NP < tokens) ? widen<T>(raw[i]) : 0.0f;
+        }
+    }
+    template <int DIRECTION> __device__ __forceinline__ void move() {
+        const char* at = reinterpret_cast<const char*>(tile);
+        const uint64_t bytes = TOKENS * (uint64_t)token_bytes;
+        tile = reinterpret_cast<const T*>(DIRECTION > 0 ? at + bytes : at - bytes);
+    }
+};
+
+// Values that are to be in registers here: the compiler would otherwise move what they are made of, and the waiting for
+// its loads, behind the loads of the next tile.
+template <uint32_t N> __device__ __forceinline__ void settle(float (&v)[N]) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) ovl_lane::keep(v[i]);
 }
-template <int S> __device__ __forceinline__ void store_states(const float (&h)[S], float* to) {
+
+// States that kernels hand to each other: padded to NP entries, four neighbouring entries of a channel side by side, then
+// the channels, so that a wavefront's accesses are dense.  S entries from entry `first` on.
+template <int S>
+__device__ __forceinline__ uint32_t state_offset(uint32_t first, uint32_t channel, uint32_t channels) {
+    return (first / 4u * channels + channel) * 4u + first % 4u;
+}
+template <int S>
+__device__ __forceinline__ void load_states(float (&h)[S], const float* from, uint32_t first, uint32_t channel, uint32_t channels) {
+    constexpr int WIDE = S >= 4 ? 4 : S;
+    typedef float vec __attribute__((ext_vector_type(WIDE)));
 #pragma unroll
-    for (int s = 0; s < S; ++s) to[s] = h[s];
+    for (int i = 0; i < S; i += WIDE) {
+        const vec v = *reinterpret_cast<const vec*>(from + state_offset<S>(first + i, channel, channels));
+#pragma unroll
+        for (int k = 0; k < WIDE; ++k) h[i + k] = v[k];
+    }
+}
+template <int S>
+__device__ __forceinline__ void store_states(const float (&h)[S], float* to, uint32_t first, uint32_t channel, uint32_t channels) {
+    constexpr int WIDE = S >= 4 ? 4 : S;
+    typedef float vec __attribute__((ext_vector_type(WIDE)));
+#pragma unroll
+    for (int i = 0; i < S; i += WIDE) {
+        vec v;
+#pragma unroll
+        for (int k = 0; k < WIDE; ++k) v[k] = h[i + k];
+        *reinterpret_cast<vec*>(to + state_offset<S>(first + i, channel, channels)) = v;
+    }
 }
 
 // S entries of a [.., state] tensor for the lane's part of the state, zero past the end.
 template <int S>
 __device__ __forceinline__ void load_entries(float (&h)[S], const float* row, uint32_t q, uint32_t n) {
+    if ((q + 1u) * S <= n) {
+        struct __attribute__((packed, aligned(4))) whole { float v[S]; };
+        const whole w = *reinterpret_cast<const whole*>(row + q * S);
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[s] = w.v[s];
+        return;
+    }
 #pragma unroll
     for (uint32_t s = 0; s < S; ++s) {
         const uint32_t at = q * S + s;
@@ -186,111 +295,239 @@ __device__ __forceinline__ float quad_pick(float x, int k) {
     }
 }
 
+// The vectors B or C of the tokens of a step for kernels with a channel per lane, where every lane needs all S entries.
+// Lane l of every row of sixteen holds entries l, l + 16, ..., and instructions take their operand from the lane of their
+// row that has it: nothing is copied, no LDS is read (sixteen registers loaded from LDS per token and vector, as broadcasts,
+// cost more than a tenth of the time).
+template <typename T, int S> struct vectors_of_step {
+    static constexpr uint32_t HELD = S <= 16 ? 1 : S / 16, IN_ROW = S < 16 ? S : 16;
+    const T* step;
+    uint32_t token_bytes, own[HELD], real;  // byte offsets; which of the lane's entries there are
+    T raw[STEP][HELD];
+    float now[STEP][HELD];
+    __device__ __forceinline__ vectors_of_step(const vectors<T>& v, const place& w, uint32_t lane, uint32_t t0, uint32_t n)
+        : step(v.data + (int64_t)w.b * v.batch_stride + (int64_t)w.g * v.group_stride + (int64_t)t0 * v.token_stride),
+          token_bytes((uint32_t)v.token_stride * (uint32_t)sizeof(T)), real(0u) {
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; ++i) {
+            const uint32_t entry = lane % 16u + 16u * i;
+            own[i] = min(entry, n - 1u) * (uint32_t)sizeof(T);
+            real |= entry < n ? 1u << i : 0u;
+        }
+    }
+    __device__ __forceinline__ void load() {
+        const ovl_lane::region r(step);
+        const uint32_t bytes = ovl_lane::anew(token_bytes);
+#pragma unroll
+        for (uint32_t j = 0; j < STEP; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) raw[j][i] = r.template load<T>(own[i], j * bytes);
+    }
+    // Only `left` tokens (at least one) are there: those behind are read as the last.
+    __device__ __forceinline__ void load_some(uint32_t left) {
+        const ovl_lane::region r(step);
+        const uint32_t bytes = ovl_lane::anew(token_bytes);
+#pragma unroll
+        for (uint32_t j = 0; j < STEP; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) raw[j][i] = r.template load<T>(own[i], min(j, left - 1u) * bytes);
+    }
+    // The loaded ones become the present ones.  Entries past the state and tokens behind the sequence (`tokens` of the step's
+    // are in it) become zero: they then add nothing anywhere.
+    __device__ __forceinline__ void take(uint32_t tokens) {
+#pragma unroll
+        for (uint32_t j = 0; j < STEP; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < HELD; ++i) {
+                now[j][i] = (real >> i & 1u) != 0u ? widen<T>(raw[j][i]) : 0.0f;
+                ovl_lane::keep(now[j][i]);
+            }
+        if (tokens < STEP)
+#pragma unroll
+            for (uint32_t j = 0; j < STEP; ++j)
+#pragma unroll
+                for (uint32_t i = 0; i < HELD; ++i) now[j][i] = j < tokens ? now[j][i] : 0.0f;
+    }
+    __device__ __forceinline__ void move() {        // to the next step
+        step = reinterpret_cast<const T*>(reinterpret_cast<const char*>(step) + STEP * (uint64_t)token_bytes);
+    }
+};
+
+// The vectors of TOKENS tokens in LDS, S entries each, read in pieces of up to 16 entries one piece ahead of their use: an
+// LDS read takes about as long as a dozen instructions.  BACKWARD: the tokens from the last.  All indexes are constants
+// once the loops are unrolled.
+template <int S, uint32_t TOKENS, bool BACKWARD> struct vector_queue {
+    static constexpr uint32_t WIDE = S < 16 ? S : 16, PIECES = S / WIDE;
+    const float* lds;
+    float held[2][WIDE];
+    __device__ __forceinline__ explicit vector_queue(const float* lds_) : lds(lds_) {}
+    __device__ __forceinline__ void read(uint32_t piece) {
+        const uint32_t token = BACKWARD ? TOKENS - 1u - piece / PIECES : piece / PIECES;
+#pragma unroll
+        for (uint32_t e = 0; e < WIDE; ++e) held[piece & 1u][e] = lds[token * S + piece % PIECES * WIDE + e];
+    }
+    __device__ __forceinline__ void begin() { read(0u); }
+    __device__ __forceinline__ void next(uint32_t j, uint32_t i) {
+        if (j * PIECES + i + 1u < TOKENS * PIECES) read(j * PIECES + i + 1u);
+    }
+    __device__ __forceinline__ float get(uint32_t j, uint32_t i, uint32_t e) const { return held[(j * PIECES + i) & 1u][e]; }
+};
+
 // ---------------------------------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------------------------------
 
+// S entries (all of a state, padded) in the lane of their channel: nothing has to be summed across lanes.  A wavefront owns
+// 64 channels and a chunk and takes STEP tokens at a time, the next ones' loads in flight.  The four wavefronts of a
+// workgroup have nothing to do with each other; they are one workgroup so that every SIMD of a compute unit gets one.
 // OUTPUT: the full pass (y, the last state, the kept states).  Otherwise only states: the chunk's own effect on a zero
 // state (`local`, `dt_sum`), or the kept states.
 template <typename T, int S, bool OUTPUT>
 __global__ void __launch_bounds__(THREADS)
-scan_forward_kernel(scan_args<T> p, uint32_t chunks, T* y, float* last, float* saved, const float* entry, float* local,
+scan_forward_kernel(scan_args<T> p, uint32_t units, uint32_t chunks, T* y, float* last, float* saved, const float* entry, float* local,
                     float* dt_sum) {
-    constexpr uint32_t NP = 4 * S;
-    __shared__ __attribute__((aligned(16))) float lds_B[2][TILE * NP];
-    __shared__ __attribute__((aligned(16))) float lds_C[OUTPUT ? 2 : 1][OUTPUT ? TILE * NP : 1];
-    const place w = find_place(p, 0u, chunks);
-    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels + w.channel;
+    typedef reader<T, STEP, 1> reads;
+    // B is taken from the lanes of a row, where it costs nothing as the factor of a product; C, a factor of a fused
+    // multiply-add, which has no such form, comes through a part of the LDS that is the wavefront's own
+    __shared__ __attribute__((aligned(16))) float lds_vectors[WAVES][OUTPUT ? 2 : 1][OUTPUT ? STEP * S : 4];
+    const uint32_t lane = threadIdx.x % 64u, wave = ovl_lane::wavefront(threadIdx.x / 64u), unit = blockIdx.x * WAVES + wave;
+    if (unit >= units) return;              // there is no barrier
+    float (*lds_C)[OUTPUT ? STEP * S : 4] = lds_vectors[wave];
+    const place w = find_place<1>(p, unit, lane, 0u, chunks);
+    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels;
     const uint64_t state_row = (uint64_t)w.b * p.channels + w.channel;
 
     float h[S], A2[S];
-    load_entries(A2, p.A + (uint64_t)w.channel * p.state, w.q, p.state);
+    load_entries(A2, p.A + (uint64_t)w.channel * p.state, 0u, p.state);
 #pragma unroll
     for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; h[s] = 0.0f; }
-    if (entry != nullptr) load_states(h, entry + chunk_row * NP + w.q * S);
-    else if (local == nullptr && p.entering != nullptr) load_entries(h, p.entering + state_row * p.state, w.q, p.state);
+    if (entry != nullptr) load_states(h, entry + chunk_row * S, 0u, w.channel, p.channels);
+    else if (local == nullptr && p.entering != nullptr) load_entries(h, p.entering + state_row * p.state, 0u, p.state);
     const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
     const float skip = OUTPUT && p.D != nullptr ? p.D[w.channel] : 0.0f;
     const bool gate = OUTPUT && p.z.data != nullptr;
     float dt_total = 0.0f;
 
-    T u_next[QUADS], delta_next[QUADS], z_next[QUADS];
-    vector_stage<T, S> B_next, C_next;
-    auto fetch = [&](uint32_t t0) {
-        load_tile(u_next, p.u, w, t0, p.length);
-        load_tile(delta_next, p.delta, w, t0, p.length);
-        if (gate) load_tile(z_next, p.z, w, t0, p.length);
-        B_next.load(p.B, w, t0, p.length, p.state);
-        if (OUTPUT) C_next.load(p.C, w, t0, p.length, p.state);
+    // tokens from `start` on; those of the sequence end before `stop`
+    const uint32_t start = w.first * TILE, stop = max(start, min(w.last * TILE, w.end)), behind = min(w.last * TILE, p.length);
+    reads u_from(p.u, w, start), delta_from(p.delta, w, start), z_from(p.z, w, start);
+    writer<T, STEP, 1> out_at(w, p.length, p.channels, start);
+    vectors_of_step<T, S> B(p.B, w, lane, start, p.state);
+    vector_stage<T, S, STEP, 64> C(p.C, w, lane, start, p.state);
+    float* kept = saved + ((uint64_t)w.b * p.tiles + w.first) * p.channels * S;
+    T u_next[STEP], delta_next[STEP], z_next[STEP], done[STEP];
+    auto fetch = [&](uint32_t left) {
+        if (left >= STEP) {
+            u_from.load(u_next);
+            delta_from.load(delta_next);
+            if (gate) z_from.load(z_next);
+            B.load();
+            if (OUTPUT) C.load();
+        } else {
+            u_from.load_some(u_next, left, 0u);
+            delta_from.load_some(delta_next, left, 0u);
+            if (gate) z_from.load_some(z_next, left, 0u);
+            B.load_some(left);
+            if (OUTPUT) C.load_some(left);
+        }
+        u_from.template move<1>();
+        delta_from.template move<1>();
+        z_from.template move<1>();
+        B.move();
+        C.template move<1>();
     };
-    if (w.first * TILE < w.end) fetch(w.first * TILE);
+    if (start < stop) fetch(p.length - start);
 
-    for (uint32_t tile = w.first; tile < w.last; ++tile) {
-        const uint32_t t0 = tile * TILE;
-        if (t0 >= w.end) {                  // behind the sequence: the state stays, the outputs are zero
-            if (OUTPUT && w.active)
+    uint32_t t0 = start;
+    for (uint32_t turn = 0; t0 < stop; t0 += STEP, turn ^= 1u) {
+        const uint32_t tokens = stop - t0;
+        B.take(tokens);
+        if (OUTPUT) C.store(lds_C[turn], tokens, p.state);
+        float u[STEP], dt[STEP], z[STEP], out[STEP];
 #pragma unroll
-                for (uint32_t j = 0; j < QUADS; ++j) {
-                    const uint32_t t = t0 + 4u * j + w.q;
-                    if (t < p.length) y[((uint64_t)w.b * p.length + t) * p.channels + w.channel] = narrow<T>(0.0f);
-                }
-            continue;
-        }
-        const uint32_t buffer = tile & 1u;
-        B_next.store(lds_B[buffer], w, t0, p.state);
-        if (OUTPUT) C_next.store(lds_C[OUTPUT ? buffer : 0], w, t0, p.state);
-        float u[QUADS], delta[QUADS], z[QUADS];
-#pragma unroll
-        for (uint32_t j = 0; j < QUADS; ++j) {
+        for (uint32_t j = 0; j < STEP; ++j) {
             u[j] = widen<T>(u_next[j]);
-            delta[j] = widen<T>(delta_next[j]) + bias;
-            z[j] = gate ? widen<T>(z_next[j]) : 0.0f;
+            dt[j] = widen<T>(delta_next[j]) + bias;
+            z[j] = 0.0f;
         }
-        // One barrier per tile: the buffer written now was last read two tiles ago, and the barrier in between has
-        // let every wavefront finish that tile.
-        __syncthreads();
-        if (tile + 1u < w.last && t0 + TILE < w.end) fetch(t0 + TILE);
-        if (saved != nullptr && w.active)
-            store_states(h, saved + (((uint64_t)w.b * p.tiles + tile) * p.channels + w.channel) * NP + w.q * S);
-
+        if (gate)
 #pragma unroll
-        for (uint32_t j = 0; j < QUADS; ++j) {
-            const uint32_t t = t0 + 4u * j + w.q;
-            const bool token = t < w.end;
-            const float dt = token ? (p.softplus ? softplus_(delta[j]) : delta[j]) : 0.0f;
-            const float uu = token ? u[j] : 0.0f;
-            const float x = dt * uu;
-            dt_total += dt;
-            float part[4];
+            for (uint32_t j = 0; j < STEP; ++j) z[j] = widen<T>(z_next[j]);
+        settle(u);
+        settle(dt);
+        settle(z);
+        if (OUTPUT) ovl_lane::wave_sync();
+        // Stores stand here, in front of the next loads: loads are waited for in the order of all memory accesses, so
+        // stores behind them would be waited for as well, right after they were issued.
+        if (OUTPUT && t0 > start) {
+            out_at.store(y, done);
+            out_at.template move<1>();
+        }
+        if (saved != nullptr && t0 % TILE == 0u) {
+            store_states(h, kept, 0u, w.channel, p.channels);
+            kept += (uint64_t)p.channels * S;
+        }
+        if (tokens > STEP) fetch(p.length - t0 - STEP);
+        if (p.softplus)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float* Bt = lds_B[buffer] + (4u * j + k) * NP + w.q * S;
-                const float* Ct = lds_C[OUTPUT ? buffer : 0] + (OUTPUT ? (4u * j + k) * NP + w.q * S : 0u);
-                const float dt_k = quad_pick(dt, k), x_k = quad_pick(x, k);
-                float sum = 0.0f;
+            for (uint32_t j = 0; j < STEP; ++j) dt[j] = softplus_(dt[j]);
+        if (tokens < STEP)
 #pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const float a = ovl_lane::exp2_(dt_k * A2[s]);
-                    h[s] = fmaf(a, h[s], x_k * Bt[s]);
-                    if (OUTPUT) sum = fmaf(Ct[s], h[s], sum);
+            for (uint32_t j = 0; j < STEP; ++j) {
+                dt[j] = j < tokens ? dt[j] : 0.0f;
+                u[j] = j < tokens ? u[j] : 0.0f;
+            }
+        // C of the next token is on its way from LDS while the present one is worked on
+        vector_queue<S, STEP, false> C_queue(lds_C[OUTPUT ? turn : 0u]);
+        if (OUTPUT) C_queue.begin();
+#pragma unroll
+        for (uint32_t j = 0; j < STEP; ++j) {
+            const float x = dt[j] * u[j];
+            if (!OUTPUT) dt_total += dt[j];
+            float sum = skip * u[j];
+#pragma unroll
+            for (uint32_t i = 0; i < B.HELD; ++i) {
+                const ovl_lane::row_values B_row(B.now[j][i]);
+                if (OUTPUT) C_queue.next(j, i);
+#pragma unroll
+                for (uint32_t e = 0; e < B.IN_ROW; ++e) {
+                    const uint32_t s = 16u * i + e;
+                    const float a = ovl_lane::exp2_(dt[j] * A2[s]);
+                    h[s] = fmaf(a, h[s], B_row.at(e) * x);
+                    if (OUTPUT) sum = fmaf(C_queue.get(j, i, e), h[s], sum);
                 }
-                part[k] = sum;
+                if (OUTPUT) __builtin_amdgcn_sched_barrier(0);
             }
-            if (OUTPUT) {
-                float out = fmaf(skip, uu, quad_scatter_sum(part, w.q));
-                if (gate) out *= z[j] * sigmoid_(z[j]);
-                if (w.active && t < p.length)
-                    y[((uint64_t)w.b * p.length + t) * p.channels + w.channel] = narrow<T>(token ? out : 0.0f);
-            }
+            out[j] = sum;
+        }
+        if (OUTPUT) {
+            if (gate)
+#pragma unroll
+                for (uint32_t j = 0; j < STEP; ++j) out[j] *= z[j] * sigmoid_(z[j]);
+            if (tokens < STEP)
+#pragma unroll
+                for (uint32_t j = 0; j < STEP; ++j) out[j] = j < tokens ? out[j] : 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < STEP; ++j) done[j] = narrow<T>(out[j]);
         }
     }
-    if (OUTPUT && w.active && w.chunk + 1u == p.chunks) store_entries(h, last + state_row * p.state, w.q, p.state);
-    if (!OUTPUT && local != nullptr) {
-        dt_total = quad_sum(dt_total);
-        if (w.active) {
-            store_states(h, local + chunk_row * NP + w.q * S);
-            if (w.q == 0u) dt_sum[chunk_row] = dt_total;
+    if (OUTPUT) {
+        if (start < stop) {                 // the last step's outputs
+            out_at.store_some(y, done, behind - (t0 - STEP), 0u);
+            out_at.template move<1>();
         }
+        T none[STEP];                       // behind the sequence the outputs are zero
+#pragma unroll
+        for (uint32_t j = 0; j < STEP; ++j) none[j] = narrow<T>(0.0f);
+        for (; t0 < behind; t0 += STEP) {
+            out_at.store_some(y, none, behind - t0, 0u);
+            out_at.template move<1>();
+        }
+    }
+    if (OUTPUT && w.chunk + 1u == p.chunks) store_entries(h, last + state_row * p.state, 0u, p.state);
+    if (!OUTPUT && local != nullptr) {
+        store_states(h, local + chunk_row * S, 0u, w.channel, p.channels);
+        dt_sum[chunk_row + w.channel] = dt_total;
     }
 }
 
@@ -301,11 +538,12 @@ template <bool REVERSE>
 __global__ void __launch_bounds__(THREADS)
 scan_join_kernel(const float* A, const float* start, float* local, const float* dt_sum, uint32_t batch, uint32_t channels,
                  uint32_t state, uint32_t padded, uint32_t chunks) {
-    const uint64_t id = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
-    if (id >= (uint64_t)batch * channels * padded) return;
-    const uint32_t n = (uint32_t)(id % padded);
-    const uint64_t row = id / padded;
-    const uint32_t channel = (uint32_t)(row % channels), b = (uint32_t)(row / channels);
+    const uint64_t id = (uint64_t)blockIdx.x * THREADS + threadIdx.x, row_size = (uint64_t)channels * padded;
+    if (id >= batch * row_size) return;
+    // the place inside a chunk's states (state_offset above), and what it stands for
+    const uint32_t b = (uint32_t)(id / row_size), in = (uint32_t)(id % row_size);
+    const uint32_t channel = in / 4u % channels, n = in / 4u / channels * 4u + in % 4u;
+    const uint64_t row = (uint64_t)b * channels + channel;
     const bool real = n < state;
     const float A2 = real ? A[(uint64_t)channel * state + n] * LOG2E : 0.0f;
     float h = real && start != nullptr ? start[row * state + n] : 0.0f;
@@ -317,16 +555,16 @@ scan_join_kernel(const float* A, const float* start, float* local, const float* 
         for (uint32_t i = 0; i < AHEAD; ++i) {
             const uint32_t step = min(base + i, chunks - 1u);
             const uint32_t chunk = REVERSE ? chunks - 1u - step : step;
-            at[i] = ((uint64_t)b * chunks + chunk) * channels + channel;
+            at[i] = (uint64_t)b * chunks + chunk;
             // the last chunk of the walk has no effect to pass on (and none was computed)
             const bool passes = step + 1u < chunks;
-            own[i] = passes ? local[at[i] * padded + n] : 0.0f;
-            sum[i] = passes ? dt_sum[at[i]] : 0.0f;
+            own[i] = passes ? local[at[i] * row_size + in] : 0.0f;
+            sum[i] = passes ? dt_sum[at[i] * channels + channel] : 0.0f;
         }
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; ++i)
             if (base + i < chunks) {
-                local[at[i] * padded + n] = h;
+                local[at[i] * row_size + in] = h;
                 h = fmaf(ovl_lane::exp2_(sum[i] * A2), h, own[i]);
             }
     }
@@ -345,67 +583,99 @@ template <typename T> struct gradient_args {
     float *vector_part, *A_part, *D_part, *bias_part;
 };
 
-// The upstream gradient of y before the gate.
-__device__ __forceinline__ float gated(float d_out, bool gate, float z) { return gate ? d_out * z * sigmoid_(z) : d_out; }
-
-// The effect of a chunk on a zero gradient entering at its end: r = a (C dy + r), tokens walked from the last.
+// The effect of a chunk on a zero gradient entering at its end: r = a (C dy + r), tokens walked from the last.  Lanes as in
+// the forward pass.
 template <typename T, int S>
 __global__ void __launch_bounds__(THREADS)
-scan_gradient_local_kernel(scan_args<T> p, sequence<T> d_y, float* local, float* dt_sum) {
-    constexpr uint32_t NP = 4 * S;
-    __shared__ __attribute__((aligned(16))) float lds_C[2][TILE * NP];
-    const place w = find_place(p, 1u, p.chunks - 1u);       // nothing enters from the first chunk
-    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels + w.channel;
+scan_gradient_local_kernel(scan_args<T> p, uint32_t units, sequence<T> d_y, float* local, float* dt_sum) {
+    typedef reader<T, STEP, 1> reads;
+    __shared__ __attribute__((aligned(16))) float lds_vectors[WAVES][2][STEP * S];
+    const uint32_t lane = threadIdx.x % 64u, wave = ovl_lane::wavefront(threadIdx.x / 64u), unit = blockIdx.x * WAVES + wave;
+    if (unit >= units) return;              // there is no barrier
+    float (*lds_C)[STEP * S] = lds_vectors[wave];
+    const place w = find_place<1>(p, unit, lane, 1u, p.chunks - 1u);       // nothing enters from the first chunk
+    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels;
     float r[S], A2[S];
-    load_entries(A2, p.A + (uint64_t)w.channel * p.state, w.q, p.state);
+    load_entries(A2, p.A + (uint64_t)w.channel * p.state, 0u, p.state);
 #pragma unroll
     for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; r[s] = 0.0f; }
     const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
     const bool gate = p.z.data != nullptr;
     float dt_total = 0.0f;
 
-    T delta_next[QUADS], z_next[QUADS], dy_next[QUADS];
-    vector_stage<T, S> C_next;
-    auto fetch = [&](uint32_t t0) {
-        load_tile(delta_next, p.delta, w, t0, p.length);
-        load_tile(dy_next, d_y, w, t0, p.length);
-        if (gate) load_tile(z_next, p.z, w, t0, p.length);
-        C_next.load(p.C, w, t0, p.length, p.state);
-    };
-    const uint32_t stop = min(w.last, (w.end + TILE - 1u) / TILE);
-    if (w.first < stop) fetch((stop - 1u) * TILE);
-    for (uint32_t tile = stop; tile-- > w.first;) {
-        const uint32_t t0 = tile * TILE, buffer = tile & 1u;
-        C_next.store(lds_C[buffer], w, t0, p.state);
-        float delta[QUADS], dy[QUADS];
-#pragma unroll
-        for (uint32_t j = 0; j < QUADS; ++j) {
-            delta[j] = widen<T>(delta_next[j]) + bias;
-            dy[j] = gated(widen<T>(dy_next[j]), gate, gate ? widen<T>(z_next[j]) : 0.0f);
+    const uint32_t start = w.first * TILE, stop = max(start, min(w.last * TILE, w.end));
+    const uint32_t steps = (stop - start + STEP - 1u) / STEP, t_last = start + (max(steps, 1u) - 1u) * STEP;
+    reads delta_from(p.delta, w, t_last), z_from(p.z, w, t_last), dy_from(d_y, w, t_last);
+    vector_stage<T, S, STEP, 64> C_next(p.C, w, lane, t_last, p.state);
+    T delta_next[STEP], z_next[STEP], dy_next[STEP];
+    auto fetch = [&](uint32_t left) {
+        if (left >= STEP) {
+            delta_from.load(delta_next);
+            dy_from.load(dy_next);
+            if (gate) z_from.load(z_next);
+            C_next.load();
+        } else {
+            delta_from.load_some(delta_next, left, 0u);
+            dy_from.load_some(dy_next, left, 0u);
+            if (gate) z_from.load_some(z_next, left, 0u);
+            C_next.load_some(left);
         }
-        __syncthreads();
-        if (tile > w.first) fetch(t0 - TILE);
+        delta_from.template move<-1>();
+        dy_from.template move<-1>();
+        z_from.template move<-1>();
+        C_next.template move<-1>();
+    };
+    if (steps > 0u) fetch(p.length - t_last);
+    for (uint32_t step = steps; step-- > 0u;) {
+        const uint32_t t0 = start + step * STEP, tokens = stop - t0, turn = step & 1u;
+        C_next.store(lds_C[turn], tokens, p.state);
+        float dt[STEP], d[STEP], z[STEP];
 #pragma unroll
-        for (uint32_t i = 0; i < QUADS; ++i) {
-            const uint32_t j = QUADS - 1u - i;
-            const bool token = t0 + 4u * j + w.q < w.end;
-            const float dt = token ? (p.softplus ? softplus_(delta[j]) : delta[j]) : 0.0f;
-            const float d = token ? dy[j] : 0.0f;
-            dt_total += dt;
+        for (uint32_t j = 0; j < STEP; ++j) {
+            dt[j] = widen<T>(delta_next[j]) + bias;
+            d[j] = widen<T>(dy_next[j]);
+            z[j] = 0.0f;
+        }
+        if (gate)
 #pragma unroll
-            for (int k = 3; k >= 0; --k) {
-                const float* Ct = lds_C[buffer] + (4u * j + k) * NP + w.q * S;
-                const float dt_k = quad_pick(dt, k), d_k = quad_pick(d, k);
+            for (uint32_t j = 0; j < STEP; ++j) z[j] = widen<T>(z_next[j]);
+        settle(dt);
+        settle(d);
+        settle(z);
+        ovl_lane::wave_sync();
+        if (step > 0u) fetch(STEP);
+        if (p.softplus)
 #pragma unroll
-                for (int s = 0; s < S; ++s) r[s] = ovl_lane::exp2_(dt_k * A2[s]) * fmaf(d_k, Ct[s], r[s]);
+            for (uint32_t j = 0; j < STEP; ++j) dt[j] = softplus_(dt[j]);
+        if (gate)
+#pragma unroll
+            for (uint32_t j = 0; j < STEP; ++j) d[j] *= z[j] * sigmoid_(z[j]);
+        if (tokens < STEP)
+#pragma unroll
+            for (uint32_t j = 0; j < STEP; ++j) {
+                dt[j] = j < tokens ? dt[j] : 0.0f;
+                d[j] = j < tokens ? d[j] : 0.0f;
+            }
+        vector_queue<S, STEP, true> C_queue(lds_C[turn]);
+        C_queue.begin();
+#pragma unroll
+        for (uint32_t k = 0; k < STEP; ++k) {
+            const uint32_t j = STEP - 1u - k;
+            dt_total += dt[j];
+#pragma unroll
+            for (uint32_t i = 0; i < C_queue.PIECES; ++i) {
+                C_queue.next(k, i);
+#pragma unroll
+                for (uint32_t e = 0; e < C_queue.WIDE; ++e) {
+                    const uint32_t s = i * C_queue.WIDE + e;
+                    r[s] = ovl_lane::exp2_(dt[j] * A2[s]) * fmaf(d[j], C_queue.get(k, i, e), r[s]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
-    dt_total = quad_sum(dt_total);
-    if (w.active) {
-        store_states(r, local + chunk_row * NP + w.q * S);
-        if (w.q == 0u) dt_sum[chunk_row] = dt_total;
-    }
+    store_states(r, local + chunk_row * S, 0u, w.channel, p.channels);
+    dt_sum[chunk_row + w.channel] = dt_total;
 }
 
 // Sums over the 16 channels of a wavefront (the quads) of 2 S values per lane and token, four tokens together.  Within a
@@ -449,45 +719,65 @@ template <int S> struct channel_sums {
     }
 };
 
-template <typename T, int S>
+template <typename T, int S, bool GATE>
 __global__ void __launch_bounds__(THREADS)
 scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, const float* entry) {
     constexpr uint32_t NP = 4 * S;
     // tokens whose states and decays are held in registers at a time
-    constexpr uint32_t SUB = S <= 4 ? 16 : S <= 8 ? 8 : 4, SUBS = TILE / SUB;
+    constexpr uint32_t SUB = S <= 2 ? 16 : S <= 4 ? 8 : 4, SUBS = TILE / SUB;
     __shared__ __attribute__((aligned(16))) float lds_B[2][TILE * NP];
     __shared__ __attribute__((aligned(16))) float lds_C[2][TILE * NP];
     __shared__ float lds_sums[WAVES][2 * TILE * NP];
-    const place w = find_place(p, 0u, p.chunks);
+    const place w = find_place<4>(p, blockIdx.x, threadIdx.x, 0u, p.chunks);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u;
-    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels + w.channel;
+    const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels;
     const uint64_t state_row = (uint64_t)w.b * p.channels + w.channel;
 
     float r[S], A2[S], dA[S];
     load_entries(A2, p.A + (uint64_t)w.channel * p.state, w.q, p.state);
 #pragma unroll
     for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; r[s] = 0.0f; dA[s] = 0.0f; }
-    if (entry != nullptr) load_states(r, entry + chunk_row * NP + w.q * S);
+    if (entry != nullptr) load_states(r, entry + chunk_row * NP, w.q * S, w.channel, p.channels);
     else if (g.d_last != nullptr) load_entries(r, g.d_last + state_row * p.state, w.q, p.state);
     const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
     const float skip = p.D != nullptr ? p.D[w.channel] : 0.0f;
-    const bool gate = p.z.data != nullptr;
     float dD = 0.0f, dbias = 0.0f;
 
+    const uint32_t stop = max(w.first, min(w.last, (w.end + TILE - 1u) / TILE)), start = (max(stop, 1u) - 1u) * TILE;
+    typedef reader<T, QUADS, 4> reads;
+    typedef writer<T, QUADS, 4> writes;
+    typedef vector_stage<T, NP, TILE, THREADS> stage;
+    reads u_from(p.u, w, start), delta_from(p.delta, w, start), z_from(p.z, w, start), dy_from(g.d_y, w, start);
+    writes out_at(w, p.length, p.channels, start);
+    stage B_next(p.B, w, threadIdx.x, start, p.state), C_next(p.C, w, threadIdx.x, start, p.state);
+    const float* kept = saved + ((uint64_t)w.b * p.tiles + start / TILE) * p.channels * NP;
     T u_next[QUADS], delta_next[QUADS], z_next[QUADS], dy_next[QUADS];
     float h_next[S];
-    vector_stage<T, S> B_next, C_next;
-    auto fetch = [&](uint32_t tile) {
-        const uint32_t t0 = tile * TILE;
-        load_tile(u_next, p.u, w, t0, p.length);
-        load_tile(delta_next, p.delta, w, t0, p.length);
-        load_tile(dy_next, g.d_y, w, t0, p.length);
-        if (gate) load_tile(z_next, p.z, w, t0, p.length);
-        load_states(h_next, saved + (((uint64_t)w.b * p.tiles + tile) * p.channels + w.channel) * NP + w.q * S);
-        B_next.load(p.B, w, t0, p.length, p.state);
-        C_next.load(p.C, w, t0, p.length, p.state);
+    auto fetch = [&](uint32_t left) {
+        if (left >= TILE) {
+            u_from.load(u_next);
+            delta_from.load(delta_next);
+            dy_from.load(dy_next);
+            if (GATE) z_from.load(z_next);
+            B_next.load();
+            C_next.load();
+        } else {
+            u_from.load_some(u_next, left, w.q);
+            delta_from.load_some(delta_next, left, w.q);
+            dy_from.load_some(dy_next, left, w.q);
+            if (GATE) z_from.load_some(z_next, left, w.q);
+            B_next.load_some(left);
+            C_next.load_some(left);
+        }
+        load_states(h_next, kept, w.q * S, w.channel, p.channels);
+        u_from.template move<-1>();
+        delta_from.template move<-1>();
+        dy_from.template move<-1>();
+        z_from.template move<-1>();
+        B_next.template move<-1>();
+        C_next.template move<-1>();
+        kept -= (uint64_t)p.channels * NP;
     };
-    const uint32_t stop = max(w.first, min(w.last, (w.end + TILE - 1u) / TILE));
     float* const part = g.vector_part + (((uint64_t)w.g * p.blocks + w.block) * p.batch + w.b) * p.length * (2u * p.state);
 
     // behind the sequence all gradients are zero
@@ -497,33 +787,63 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
             const uint64_t at = ((uint64_t)w.b * p.length + t) * p.channels + w.g * p.per_group + c;
             g.d_u[at] = narrow<T>(0.0f);
             g.d_delta[at] = narrow<T>(0.0f);
-            if (gate) g.d_z[at] = narrow<T>(0.0f);
+            if (GATE) g.d_z[at] = narrow<T>(0.0f);
         }
         for (uint32_t n = threadIdx.x % BLOCK; n < 2u * p.state; n += BLOCK) part[(uint64_t)t * 2u * p.state + n] = 0.0f;
     }
 
-    if (w.first < stop) fetch(stop - 1u);
     for (uint32_t tile = stop; tile-- > w.first;) {
-        const uint32_t t0 = tile * TILE, buffer = tile & 1u;
-        B_next.store(lds_B[buffer], w, t0, p.state);
-        C_next.store(lds_C[buffer], w, t0, p.state);
-        float u[QUADS], raw[QUADS], dt[QUADS], x[QUADS], z[QUADS], d_out[QUADS], d[QUADS], h[SUBS][S];
+        const uint32_t t0 = tile * TILE, buffer = tile & 1u, left = p.length - t0, tokens = w.end - t0;
+        T du_done[QUADS], ddelta_done[QUADS], dz_done[QUADS];
+        // Loaded here and not a tile ahead: the registers for that cost the second wavefront of a SIMD, which hides more
+        // (261 registers and one wavefront: 690 us, 247 and two: 540 us for 4 x 2048 tokens of 4096 channels).
+        fetch(left);
+        B_next.store(lds_B[buffer], tokens, p.state);
+        C_next.store(lds_C[buffer], tokens, p.state);
+        float u[QUADS], dt[QUADS], x[QUADS], d[QUADS], h[SUBS][S];
+        float slope[QUADS], gate_slope[QUADS];              // d dt / d delta; d z is gate_slope times y
 #pragma unroll
         for (uint32_t j = 0; j < QUADS; ++j) {
-            const bool token = t0 + 4u * j + w.q < w.end;
-            u[j] = token ? widen<T>(u_next[j]) : 0.0f;
-            raw[j] = widen<T>(delta_next[j]) + bias;
-            dt[j] = token ? (p.softplus ? softplus_(raw[j]) : raw[j]) : 0.0f;
-            x[j] = dt[j] * u[j];
-            z[j] = gate ? widen<T>(z_next[j]) : 0.0f;
-            d_out[j] = token ? widen<T>(dy_next[j]) : 0.0f;
-            d[j] = token ? gated(d_out[j], gate, z[j]) : 0.0f;
+            // lanes without a channel of their own add nothing to any sum
+            u[j] = w.active ? widen<T>(u_next[j]) : 0.0f;
+            dt[j] = widen<T>(delta_next[j]) + bias;
+            d[j] = w.active ? widen<T>(dy_next[j]) : 0.0f;
+            gate_slope[j] = GATE ? widen<T>(z_next[j]) : 0.0f;
         }
 #pragma unroll
         for (int s = 0; s < S; ++s) h[0][s] = h_next[s];
         // also lets every wavefront finish reading lds_sums of the tile before
         __syncthreads();
-        if (tile > w.first) fetch(tile - 1u);
+        if (tokens < TILE)
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) {
+                u[j] = 4u * j + w.q < tokens ? u[j] : 0.0f;
+                d[j] = 4u * j + w.q < tokens ? d[j] : 0.0f;
+                gate_slope[j] = 4u * j + w.q < tokens ? gate_slope[j] : 0.0f;
+            }
+        if (GATE)
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) {
+                const float z = gate_slope[j], s = sigmoid_(z), d_out = d[j];
+                d[j] = d_out * z * s;
+                gate_slope[j] = d_out * s * fmaf(z, 1.0f - s, 1.0f);
+            }
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) slope[j] = 1.0f;
+        if (p.softplus)
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) {
+                slope[j] = sigmoid_(dt[j]);
+                dt[j] = softplus_(dt[j]);
+            }
+        if (tokens < TILE)
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) dt[j] = 4u * j + w.q < tokens ? dt[j] : 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+            x[j] = dt[j] * u[j];
+            dD = fmaf(d[j], u[j], dD);
+        }
 
         // the states that enter the later parts of the tile
 #pragma unroll
@@ -538,6 +858,7 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
 #pragma unroll
                 for (int s = 0; s < S; ++s)
                     h[part_of + 1u][s] = fmaf(ovl_lane::exp2_(dt_k * A2[s]), h[part_of + 1u][s], x_k * Bt[s]);
+                if (at % 4u == 3u) __builtin_amdgcn_sched_barrier(0);
             }
         }
 
@@ -564,10 +885,12 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
                     for (int s = 0; s < S; ++s) {
                         a[i + k][s] = ovl_lane::exp2_(dt_k * A2[s]);
                         state[i + k + 1][s] = fmaf(a[i + k][s], state[i + k][s], x_k * Bt[s]);
-                        if (gate) sums[k] = fmaf(Ct[s], state[i + k + 1][s], sums[k]);
+                        if (GATE) sums[k] = fmaf(Ct[s], state[i + k + 1][s], sums[k]);
                     }
                 }
-                y[i / 4u] = gate ? fmaf(skip, u[j], quad_scatter_sum(sums, w.q)) : 0.0f;
+                y[i / 4u] = GATE ? fmaf(skip, u[j], quad_scatter_sum(sums, w.q)) : 0.0f;
+                // (keeps the scheduler from loading B and C of all tokens at once)
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (uint32_t step = 0; step < SUB; step += 4u) {
@@ -593,31 +916,36 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
                         dA_tile[s] = fmaf(dt_k, moved, dA_tile[s]);
                         through[k] = fmaf(moved, A2[s], through[k]);
                     }
-                    // lanes without a channel add nothing
-#pragma unroll
-                    for (int s = 0; s < S; ++s) { dB[s] = w.active ? dB[s] : 0.0f; dC[s] = w.active ? dC[s] : 0.0f; }
                     sums.add(dB, dC, k, lane);
                 }
                 sums.put(lds_sums[wave], 4u * j, lane);
-                const uint32_t t = t0 + 4u * j + w.q;
-                const bool token = t < w.end;
                 const float d_x = quad_scatter_sum(dx, w.q);
-                float d_dt = fmaf(d_x, u[j], LN2 * quad_scatter_sum(through, w.q));
-                if (p.softplus) d_dt *= sigmoid_(raw[j]);
-                d_dt = token ? d_dt : 0.0f;
+                float d_dt = fmaf(d_x, u[j], LN2 * quad_scatter_sum(through, w.q)) * slope[j];
+                if (tokens < TILE) d_dt = 4u * j + w.q < tokens ? d_dt : 0.0f;
                 dbias += d_dt;
-                dD = fmaf(d[j], u[j], dD);
-                if (w.active && t < p.length) {
-                    const uint64_t at = ((uint64_t)w.b * p.length + t) * p.channels + w.channel;
-                    g.d_u[at] = narrow<T>(token ? fmaf(d_x, dt[j], skip * d[j]) : 0.0f);
-                    g.d_delta[at] = narrow<T>(d_dt);
-                    if (gate) {
-                        const float s = sigmoid_(z[j]);
-                        g.d_z[at] = narrow<T>(token ? d_out[j] * y[i / 4u] * s * fmaf(z[j], 1.0f - s, 1.0f) : 0.0f);
-                    }
-                }
+                du_done[j] = narrow<T>(fmaf(d_x, dt[j], skip * d[j]));
+                ddelta_done[j] = narrow<T>(d_dt);
+                if (GATE) dz_done[j] = narrow<T>(gate_slope[j] * y[i / 4u]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if (tokens < TILE)
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) {
+                du_done[j] = 4u * j + w.q < tokens ? du_done[j] : narrow<T>(0.0f);
+                if (GATE) dz_done[j] = 4u * j + w.q < tokens ? dz_done[j] : narrow<T>(0.0f);
+            }
+        if (!w.active) {
+        } else if (left >= TILE) {
+            out_at.store(g.d_u, du_done);
+            out_at.store(g.d_delta, ddelta_done);
+            if (GATE) out_at.store(g.d_z, dz_done);
+        } else {
+            out_at.store_some(g.d_u, du_done, left, w.q);
+            out_at.store_some(g.d_delta, ddelta_done, left, w.q);
+            if (GATE) out_at.store_some(g.d_z, dz_done, left, w.q);
+        }
+        out_at.template move<-1>();
 #pragma unroll
         for (int s = 0; s < S; ++s) dA[s] += dA_tile[s];
 
@@ -625,23 +953,21 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
         __syncthreads();
         for (uint32_t at = threadIdx.x; at < 2u * TILE * NP; at += THREADS) {
             const uint32_t set = at / (TILE * NP), t = at / NP % TILE, n = at % NP;
-            if (n < p.state && t0 + t < p.length) {
-                float sum = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
-                for (uint32_t v = 0; v < WAVES; ++v) sum += lds_sums[v][at];
-                part[(uint64_t)(t0 + t) * 2u * p.state + set * p.state + n] = t0 + t < w.end ? sum : 0.0f;
-            }
+            for (uint32_t v = 0; v < WAVES; ++v) sum += lds_sums[v][at];
+            if (n < p.state && t < left) part[(uint64_t)(t0 + t) * 2u * p.state + set * p.state + n] = t < tokens ? sum : 0.0f;
         }
     }
     if (w.active) {
-        store_states(dA, g.A_part + chunk_row * NP + w.q * S);
+        store_states(dA, g.A_part + chunk_row * NP, w.q * S, w.channel, p.channels);
         if (w.chunk == 0u && g.d_entering != nullptr) store_entries(r, g.d_entering + state_row * p.state, w.q, p.state);
     }
     dD = quad_sum(dD);
     dbias = quad_sum(dbias);
     if (w.active && w.q == 0u) {
-        g.D_part[chunk_row] = dD;
-        g.bias_part[chunk_row] = dbias;
+        g.D_part[chunk_row + w.channel] = dD;
+        g.bias_part[chunk_row + w.channel] = dbias;
     }
 }
 
@@ -677,7 +1003,7 @@ scan_gradient_sum_kernel(const float* vector_part, const float* A_part, const fl
     float sum = 0.0f;
     if (n < state) {
 #pragma unroll 8
-        for (uint32_t k = 0; k < rows; ++k) sum += A_part[((uint64_t)k * channels + channel) * padded + n];
+        for (uint32_t k = 0; k < rows; ++k) sum += A_part[(uint64_t)k * channels * padded + state_offset<1>(n, (uint32_t)channel, channels)];
         d_A[channel * state + n] = sum;
     } else if ((n == state ? d_D : d_bias) != nullptr) {
         const float* from = n == state ? D_part : bias_part;
@@ -776,7 +1102,7 @@ struct plan {
 
 // Into how many chunks the length is split.
 void chunks_for(plan& p) {
-    constexpr uint64_t ENOUGH = 192, WANTED = 1024;
+    constexpr uint64_t ENOUGH = 1024, WANTED = 1024 * RESIDENT;
     constexpr uint32_t SHORTEST = 4;        // tiles per chunk
     p.chunks = 1;
     if (p.strands < ENOUGH) {
@@ -804,6 +1130,11 @@ int check(const char* who, const ovl_ssm_scan* s, bool token, plan& p) {
     if (token && (s->length != 1u || s->lengths != nullptr))
         return fail(OVL_SSM_EINVAL, name + ": a step takes one token of every sequence");
     if (s->length > (1u << 30)) return fail(OVL_SSM_EINVAL, name + ": length must be at most 2^30");
+    // a lane's offset inside a tile has 32 bits
+    if (s->channels > (1u << 22)) return fail(OVL_SSM_EINVAL, name + ": at most 2^22 channels");
+    for (const int64_t stride : {s->u.token_stride, s->delta.token_stride, s->z.token_stride, s->B.token_stride, s->C.token_stride})
+        if (!token && s->length > 1u && (stride < 0 || stride > OVL_SSM_MAX_TOKEN_STRIDE))
+            return fail(OVL_SSM_EINVAL, name + ": token strides must be 0 to 2^25 elements");
     p.entries = entries_of(s->state);
     p.per_group = s->channels / s->groups;
     p.blocks = (p.per_group + BLOCK - 1u) / BLOCK;
@@ -858,26 +1189,31 @@ void join(const ovl_ssm_scan* s, const plan& p, const float* start, float* local
                        s->A, start, local, dt_sum, s->batch, s->channels, s->state, 4u * p.entries, p.chunks);
 }
 
-template <typename T, int S>
+// Workgroups of kernels whose wavefronts take a unit each.
+dim3 groups_of(uint64_t units) { return dim3((uint32_t)((units + WAVES - 1) / WAVES)); }
+
+// ENTRIES: state entries per lane of a quad; a lane with a channel of its own holds four times as many.
+template <typename T, int ENTRIES>
 void forward(const ovl_ssm_scan* s, const plan& p, T* y, float* last, float* saved, float* scratch, hipStream_t stream) {
+    constexpr int S = 4 * ENTRIES;
     const scan_args<T> args = make_args<T>(s, p);
     const layout at = lay_out(s, p, false);
     const float* entry = nullptr;
     if (p.chunks > 1u) {
         float* local = scratch + at.local;
         float* dt_sum = scratch + at.dt_sum;
-        hipLaunchKernelGGL((scan_forward_kernel<T, S, false>), dim3((uint32_t)(p.strands * (p.chunks - 1u))), dim3(THREADS), 0,
-                           stream, args, p.chunks - 1u, static_cast<T*>(nullptr), static_cast<float*>(nullptr),
+        hipLaunchKernelGGL((scan_forward_kernel<T, S, false>), groups_of(p.strands * (p.chunks - 1u)), dim3(THREADS), 0,
+                           stream, args, (uint32_t)(p.strands * (p.chunks - 1u)), p.chunks - 1u, static_cast<T*>(nullptr), static_cast<float*>(nullptr),
                            static_cast<float*>(nullptr), static_cast<const float*>(nullptr), local, dt_sum);
         join<false>(s, p, s->entering, local, dt_sum, stream);
         entry = local;
     }
-    const dim3 grid((uint32_t)(p.strands * p.chunks));
+    const uint32_t units = (uint32_t)(p.strands * p.chunks);
     if (y != nullptr)
-        hipLaunchKernelGGL((scan_forward_kernel<T, S, true>), grid, dim3(THREADS), 0, stream, args, p.chunks, y, last, saved,
+        hipLaunchKernelGGL((scan_forward_kernel<T, S, true>), groups_of(units), dim3(THREADS), 0, stream, args, units, p.chunks, y, last, saved,
                            entry, static_cast<float*>(nullptr), static_cast<float*>(nullptr));
     else
-        hipLaunchKernelGGL((scan_forward_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, p.chunks, y, last, saved,
+        hipLaunchKernelGGL((scan_forward_kernel<T, S, false>), groups_of(units), dim3(THREADS), 0, stream, args, units, p.chunks, y, last, saved,
                            entry, static_cast<float*>(nullptr), static_cast<float*>(nullptr));
 }
 
@@ -901,13 +1237,16 @@ void backward(const ovl_ssm_scan* s, const plan& p, const float* saved, const ov
     if (p.chunks > 1u) {
         float* local = scratch + at.local;
         float* dt_sum = scratch + at.dt_sum;
-        hipLaunchKernelGGL((scan_gradient_local_kernel<T, S>), dim3((uint32_t)(p.strands * (p.chunks - 1u))), dim3(THREADS), 0,
-                           stream, args, to.d_y, local, dt_sum);
+        hipLaunchKernelGGL((scan_gradient_local_kernel<T, 4 * S>), groups_of(p.strands * (p.chunks - 1u)), dim3(THREADS), 0,
+                           stream, args, (uint32_t)(p.strands * (p.chunks - 1u)), to.d_y, local, dt_sum);
         join<true>(s, p, g->d_last, local, dt_sum, stream);
         entry = local;
     }
-    hipLaunchKernelGGL((scan_backward_kernel<T, S>), dim3((uint32_t)(p.strands * p.chunks)), dim3(THREADS), 0, stream, args, to,
-                       saved, entry);
+    const dim3 grid((uint32_t)(p.strands * p.chunks));
+    if (s->z.data != nullptr)
+        hipLaunchKernelGGL((scan_backward_kernel<T, S, true>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
+    else
+        hipLaunchKernelGGL((scan_backward_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
     const uint64_t vector_all = (uint64_t)s->groups * s->batch * s->length * 2u * s->state;
     const uint32_t vector_groups = (uint32_t)((vector_all + THREADS - 1) / THREADS);
     const uint32_t rest = (uint32_t)(((uint64_t)s->channels * (s->state + 2u) + THREADS - 1) / THREADS);
@@ -982,6 +1321,8 @@ int ovl_ssm_scan_backward(const ovl_ssm_scan* s, const float* saved, const ovl_s
     if (g == nullptr || saved == nullptr || g->d_y.data == nullptr || g->d_u == nullptr || g->d_delta == nullptr ||
         g->d_B == nullptr || g->d_C == nullptr || g->d_A == nullptr || (s->z.data != nullptr && g->d_z == nullptr))
         return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_backward: null tensor");
+    if (s->length > 1u && (g->d_y.token_stride < 0 || g->d_y.token_stride > OVL_SSM_MAX_TOKEN_STRIDE))
+        return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_backward: token strides must be 0 to 2^25 elements");
     if (workspace == nullptr || workspace_bytes < lay_out(s, p, true).all * sizeof(float) || !aligned16(workspace))
         return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_backward: workspace too small or not 16-byte aligned");
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);

@@ -34,6 +34,8 @@ EXPORTED_SYMBOLS = ('ovl_ssm_scan_workspace_bytes', 'ovl_ssm_scan_saved_bytes', 
 
 #: largest number of state entries per channel, and of taps of the convolution
 MAX_STATE, MAX_WIDTH = 64, 4
+#: largest token stride (in elements) the scan takes as it is; tensors with larger ones are copied
+MAX_TOKEN_STRIDE = 1 << 25
 
 
 def build(force=False):
@@ -183,7 +185,7 @@ class _Arguments(object):
         return t
 
     def side_by_side(self, t):
-        if t.stride(-1) != 1 and t.shape[-1] != 1:
+        if (t.stride(-1) != 1 and t.shape[-1] != 1) or (t.dim() > 2 and t.stride(1) > MAX_TOKEN_STRIDE):
             t = t.contiguous()
             self.kept.append(t)
         return t

@@ -66,6 +66,21 @@ static inline float log2_(float x) { return log2f(x); }
 static inline float rcp_(float x) { return 1.0f / x; }
 static inline float rsq_(float x) { return 1.0f / sqrtf(x); }
 
+static inline float positive(float x) { return x > 0.0f ? x : 0.0f; }
+static inline void keep(float&) {}
+static inline uint32_t anew(uint32_t x) { return x; }
+
+static inline uint32_t wavefront(uint32_t x) { return x; }
+
+static inline void wave_sync() { pthread_barrier_wait(&ovl_emulated_wave_barrier[threadIdx.x / 64u]); }
+
+struct region {
+    char* base;
+    explicit region(const void* base_) : base(const_cast<char*>(static_cast<const char*>(base_))) {}
+    template <typename T> T load(uint32_t own, uint32_t shared) const { return *reinterpret_cast<const T*>(base + own + (uint64_t)shared); }
+    template <typename T> void store(T x, uint32_t own, uint32_t shared) const { *reinterpret_cast<T*>(base + own + (uint64_t)shared) = x; }
+};
+
 // The value `from` names, by lane; zero where it is negative.
 template <typename F> static inline float move(float x, F from) {
     const uint32_t t = threadIdx.x, wave = t / 64u, lane = t % 64u;
@@ -85,6 +100,18 @@ template <int N> static inline float row_up(float x) { return move(x, [](int l) 
 template <int N> static inline float row_round(float x) {
     return move(x, [](int l) { return (l & ~15) + ((l + 16 - N) & 15); });
 }
+
+struct row_values {
+    float all[16];
+    explicit row_values(float x) {
+        const uint32_t t = threadIdx.x, wave = t / 64u;
+        ovl_emulated_lane_values[t] = bits_of(x);
+        pthread_barrier_wait(&ovl_emulated_wave_barrier[wave]);
+        for (uint32_t n = 0; n < 16u; ++n) all[n] = float_of((uint32_t)ovl_emulated_lane_values[t / 16u * 16u + n]);
+        pthread_barrier_wait(&ovl_emulated_wave_barrier[wave]);
+    }
+    float at(uint32_t n) const { return all[n]; }
+};
 
 static inline void swap_halves(float& a, float& b) {
     const uint32_t lane = threadIdx.x % 64u;

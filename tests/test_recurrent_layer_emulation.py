@@ -33,9 +33,11 @@ def program():
         with open(path) as f:
             headers += f.read()
     # the name of the program depends on the sources' text: the stand-in header is part of it
-    parts[-1] += '\n// ' + hashlib.sha224(headers.encode('utf-8')).hexdigest() + '\n'
+    parts[-1] += '\n// one stack per thread ' + hashlib.sha224(headers.encode('utf-8')).hexdigest() + '\n'
     include = os.path.normpath(os.path.join(local.csrc_directory, '..', '..', 'include'))
-    return host_emulation.build_source(parts, 'emu_recurrent_layer', ['-I' + include])
+    # (one stack per thread: the sanitizer's second ones, for returned frames, exhaust the mappings a process may have)
+    return host_emulation.build_source(parts, 'emu_recurrent_layer',
+                                       ['-I' + include, '-fsanitize-address-use-after-return=never'])
 
 
 def to_numpy(t):
