@@ -38,7 +38,6 @@ constexpr uint32_t WAVES = 4;
 constexpr uint32_t THREADS = 64 * WAVES;
 constexpr uint32_t BLOCK = 64;              // channels of a workgroup
 constexpr uint32_t STEP = 8;                // tokens that a lane with a channel of its own takes at a time
-constexpr int RESIDENT = 2;                 // wavefronts of the kernels with a channel per lane on a SIMD
 
 constexpr float LOG2E = 0x1.715476p+0f, LN2 = 0x1.62e43p-1f;
 
@@ -531,15 +530,25 @@ scan_forward_kernel(scan_args<T> p, uint32_t units, uint32_t chunks, T* y, float
     }
 }
 
-// Joins the chunks: in place of each chunk's own effect `local` the state that enters it.  One thread per (sequence,
-// channel, state entry).  REVERSE: the gradient's recurrence, which enters chunks from their ends.  Eight chunks are read
-// before they are overwritten, so that the loads do not wait for one another.
+// Joins the chunks: in place of each chunk's own effect `local` the state that enters it.  A thread takes AHEAD chunks of a
+// (sequence, channel, state entry) in a row, which it reads before any is overwritten, and `walkers` threads (a power of
+// two) stand behind one another: each makes one step (decay, effect) of its chunks, the states between them are joined
+// through LDS, and each hands its own state on.  So 128 chunks are one trip of 16 walkers, where a thread alone would wait
+// for memory 16 times (2048 channels of 16 entries: 19.6 us, now JOIN_US).  REVERSE: the gradient's recurrence, which
+// enters chunks from their ends.
+constexpr uint32_t AHEAD = 8, MOST_WALKERS = 16;
+constexpr uint32_t join_ids(uint32_t walkers) { return walkers < 4u ? THREADS / walkers : 64u; }
+
 template <bool REVERSE>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(64 * MOST_WALKERS)
 scan_join_kernel(const float* A, const float* start, float* local, const float* dt_sum, uint32_t batch, uint32_t channels,
-                 uint32_t state, uint32_t padded, uint32_t chunks) {
-    const uint64_t id = (uint64_t)blockIdx.x * THREADS + threadIdx.x, row_size = (uint64_t)channels * padded;
-    if (id >= batch * row_size) return;
+                 uint32_t state, uint32_t padded, uint32_t chunks, uint32_t walkers) {
+    __shared__ float lds_step[2][64 * MOST_WALKERS];
+    const uint32_t ids = join_ids(walkers), column = threadIdx.x % ids;
+    const uint32_t walker = ovl_lane::wavefront(threadIdx.x / 64u) * 64u / ids;
+    const uint64_t row_size = (uint64_t)channels * padded, all = batch * row_size;
+    // threads behind the last entry repeat it, but do not write
+    const uint64_t wanted = (uint64_t)blockIdx.x * ids + column, id = wanted < all ? wanted : all - 1u;
     // the place inside a chunk's states (state_offset above), and what it stands for
     const uint32_t b = (uint32_t)(id / row_size), in = (uint32_t)(id % row_size);
     const uint32_t channel = in / 4u % channels, n = in / 4u / channels * 4u + in % 4u;
@@ -547,9 +556,9 @@ scan_join_kernel(const float* A, const float* start, float* local, const float* 
     const bool real = n < state;
     const float A2 = real ? A[(uint64_t)channel * state + n] * LOG2E : 0.0f;
     float h = real && start != nullptr ? start[row * state + n] : 0.0f;
-    constexpr uint32_t AHEAD = 8;
-    for (uint32_t base = 0; base < chunks; base += AHEAD) {
-        float own[AHEAD], sum[AHEAD];
+    for (uint32_t trip = 0; trip < chunks; trip += walkers * AHEAD) {
+        const uint32_t base = trip + walker * AHEAD;
+        float own[AHEAD], decay[AHEAD];
         uint64_t at[AHEAD];
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; ++i) {
@@ -559,13 +568,35 @@ scan_join_kernel(const float* A, const float* start, float* local, const float* 
             // the last chunk of the walk has no effect to pass on (and none was computed)
             const bool passes = step + 1u < chunks;
             own[i] = passes ? local[at[i] * row_size + in] : 0.0f;
-            sum[i] = passes ? dt_sum[at[i] * channels + channel] : 0.0f;
+            decay[i] = passes ? dt_sum[at[i] * channels + channel] : 0.0f;
+        }
+        float effect = 0.0f, factor = 1.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            decay[i] = ovl_lane::exp2_(decay[i] * A2);
+            effect = fmaf(decay[i], effect, own[i]);
+            factor *= decay[i];
+        }
+        if (walkers > 1u) {
+            lds_step[0][threadIdx.x] = factor;
+            lds_step[1][threadIdx.x] = effect;
+            __syncthreads();                // also: every chunk of the trip has been read
+        }
+        float mine = h;
+        for (uint32_t before = 0; before < walker; ++before)
+            mine = fmaf(lds_step[0][before * ids + column], mine, lds_step[1][before * ids + column]);
+        if (walkers > 1u) {
+            for (uint32_t other = 0; other < walkers; ++other)
+                h = fmaf(lds_step[0][other * ids + column], h, lds_step[1][other * ids + column]);
+            __syncthreads();
+        } else {
+            h = fmaf(factor, h, effect);
         }
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; ++i)
             if (base + i < chunks) {
-                local[at[i] * row_size + in] = h;
-                h = fmaf(ovl_lane::exp2_(sum[i] * A2), h, own[i]);
+                if (wanted < all) local[at[i] * row_size + in] = mine;
+                mine = fmaf(decay[i], mine, own[i]);
             }
     }
 }
@@ -1102,8 +1133,8 @@ struct plan {
 
 // Into how many chunks the length is split.
 void chunks_for(plan& p) {
-    constexpr uint64_t ENOUGH = 1024, WANTED = 1024 * RESIDENT;
-    constexpr uint32_t SHORTEST = 4;        // tiles per chunk
+    constexpr uint64_t ENOUGH = 1024, WANTED = 4096;
+    constexpr uint32_t SHORTEST = 1;        // tiles per chunk
     p.chunks = 1;
     if (p.strands < ENOUGH) {
         const uint64_t wanted = (WANTED + p.strands - 1) / p.strands;
@@ -1185,8 +1216,11 @@ layout lay_out(const ovl_ssm_scan* s, const plan& p, bool backward) {
 template <bool REVERSE>
 void join(const ovl_ssm_scan* s, const plan& p, const float* start, float* local, const float* dt_sum, hipStream_t stream) {
     const uint64_t all = (uint64_t)s->batch * s->channels * 4u * p.entries;
-    hipLaunchKernelGGL((scan_join_kernel<REVERSE>), dim3((uint32_t)((all + THREADS - 1) / THREADS)), dim3(THREADS), 0, stream,
-                       s->A, start, local, dt_sum, s->batch, s->channels, s->state, 4u * p.entries, p.chunks);
+    uint32_t walkers = 1;
+    while (walkers < MOST_WALKERS && walkers * AHEAD < p.chunks) walkers *= 2u;
+    const uint32_t ids = join_ids(walkers);
+    hipLaunchKernelGGL((scan_join_kernel<REVERSE>), dim3((uint32_t)((all + ids - 1) / ids)), dim3(ids * walkers), 0, stream,
+                       s->A, start, local, dt_sum, s->batch, s->channels, s->state, 4u * p.entries, p.chunks, walkers);
 }
 
 // Workgroups of kernels whose wavefronts take a unit each.
