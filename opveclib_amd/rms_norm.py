@@ -8,8 +8,10 @@ beside rows of 16 bits.  Sums and statistics are float32.  Launches go to the cu
 synchronise; equal calls give equal bits.
 """
 
+import contextlib
 import ctypes
 import os
+import struct
 import subprocess
 
 from . import local
@@ -49,6 +51,11 @@ class Norm(ctypes.Structure):
                 ('residual_dtype', ctypes.c_int32), ('weight_dtype', ctypes.c_int32), ('eps', ctypes.c_float),
                 ('x', ctypes.c_void_p), ('x_stride', ctypes.c_int64), ('residual', ctypes.c_void_p),
                 ('residual_stride', ctypes.c_int64), ('weight', ctypes.c_void_p)]
+
+
+# Packer of the struct above for the calls below: filling a ctypes structure costs ten times as much as packing its fields
+# into a bytes object.
+_pack = struct.Struct('@5If5Q').pack
 
 
 _lib = None
@@ -113,17 +120,18 @@ def _rows(t):
 def _check(torch, t, name, like, dtypes):
     if not isinstance(t, torch.Tensor):
         raise TypeError(name + ' must be a torch tensor')
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise TypeError('%s is on %s, expected %s' % (name, t.device, like.device))
     if t.dtype not in dtypes:
         raise TypeError('%s must be %s, got %s' % (name, ' or '.join(str(d) for d in dtypes), t.dtype))
 
 
 def _describe(torch, x, weight, eps, residual):
-    """The call's struct, and the tensors it points at."""
+    """The numbers in front of the addresses in ``ovl_norm``, and (rows, row stride) of x, (rows, row stride) of the
+    residual - (None, 0) without one - and the dense weight."""
     if not isinstance(x, torch.Tensor):
         raise TypeError('x must be a torch tensor')
-    if x.device.type != 'cuda':
+    if not x.is_cuda:
         raise RuntimeError('the norm kernels run on an AMD GPU: tensors must live on a HIP device')
     code = _type_code(x.dtype, 'x')
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_COLUMNS:
@@ -131,27 +139,38 @@ def _describe(torch, x, weight, eps, residual):
     columns = x.shape[-1]
     types = (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32)
     _check(torch, weight, 'weight', x, types)
-    if tuple(weight.shape) != (columns,):
+    if weight.shape != (columns,):
         raise TypeError('weight must be [%d], got %s' % (columns, list(weight.shape)))
-    weight = weight.contiguous()
-    rows, stride = _rows(x)
-    other, other_stride, other_code = None, 0, code
+    other, other_code = (None, 0), code
     if residual is not None:
         _check(torch, residual, 'residual', x, types)
         if residual.shape != x.shape:
             raise TypeError('residual must be %s, got %s' % (list(x.shape), list(residual.shape)))
-        other, other_stride = _rows(residual)
+        other = _rows(residual)
         other_code = _codes[residual.dtype]
-    norm = Norm(x.numel() // columns, columns, code, other_code, _codes[weight.dtype], float(eps), rows.data_ptr(), stride,
-                None if other is None else other.data_ptr(), other_stride, weight.data_ptr())
-    return norm, (rows, other, weight)
+    if x.numel() // columns >= 1 << 32:
+        raise TypeError('x must have fewer than 2^32 rows, got %s' % list(x.shape))
+    numbers = (x.numel() // columns, columns, code, other_code, _codes[weight.dtype], eps)
+    return numbers, _rows(x), other, weight.contiguous()
 
 
-def _on(torch, device):
-    import contextlib
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _norm(numbers, rows, other, weight):
+    """``ovl_norm`` as bytes."""
+    return _pack(*numbers, rows[0].data_ptr(), rows[1], 0 if other[0] is None else other[0].data_ptr(), other[1],
+                 weight.data_ptr())
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(torch, index):
+    """The device of the call as the current one; without the cost of switching where it is already."""
+    return _here if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _new(torch, like):
+    """A dense tensor of that shape and type for a result."""
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 def rms_norm(x, weight, eps=1e-5, residual=None):
@@ -164,13 +183,13 @@ def rms_norm(x, weight, eps=1e-5, residual=None):
     :return: y like ``x``; with a residual (y, s)
     """
     import torch
-    norm, held = _describe(torch, x, weight, eps, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    summed = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    if norm.rows > 0:
-        with _on(torch, x.device):
-            _call(library().ovl_norm_forward(ctypes.byref(norm), y.data_ptr(), None if summed is None else summed.data_ptr(),
-                                             torch.cuda.current_stream(x.device).cuda_stream))
+    held = _describe(torch, x, weight, eps, residual)
+    y = _new(torch, x)
+    summed = None if residual is None else _new(torch, residual)
+    if x.numel() > 0:
+        with _on(torch, x.get_device()):
+            _call(library().ovl_norm_forward(_norm(*held), y.data_ptr(), None if summed is None else summed.data_ptr(),
+                                             torch._C._cuda_getCurrentRawStream(x.get_device())))
     return y if residual is None else (y, summed)
 
 
@@ -186,16 +205,16 @@ def rms_norm_quantized(x, weight, eps=1e-5, residual=None, group=None):
     import torch
     if group not in (None, GROUP_COLUMNS):
         raise ValueError('group must be None or %d, got %r' % (GROUP_COLUMNS, group))
-    norm, held = _describe(torch, x, weight, eps, residual)
+    held = _describe(torch, x, weight, eps, residual)
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    groups = 1 if group is None else -(-norm.columns // group)
+    groups = 1 if group is None else -(-x.shape[-1] // group)
     scales = torch.empty(x.shape[:-1] + (groups,), dtype=torch.float32, device=x.device)
-    summed = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    if norm.rows > 0:
-        with _on(torch, x.device):
-            _call(library().ovl_norm_forward_quantized(ctypes.byref(norm), group or 0, q.data_ptr(), scales.data_ptr(),
+    summed = None if residual is None else _new(torch, residual)
+    if x.numel() > 0:
+        with _on(torch, x.get_device()):
+            _call(library().ovl_norm_forward_quantized(_norm(*held), group or 0, q.data_ptr(), scales.data_ptr(),
                                                        None if summed is None else summed.data_ptr(),
-                                                       torch.cuda.current_stream(x.device).cuda_stream))
+                                                       torch._C._cuda_getCurrentRawStream(x.get_device())))
     return (q, scales) if residual is None else (q, scales, summed)
 
 
@@ -216,31 +235,29 @@ def rms_norm_grad(s, weight, d_y, d_s=None, eps=1e-5, both=False):
     _check(torch, s, 's', d_y, types)
     if d_y.shape != s.shape:
         raise TypeError('d_y must be %s, got %s' % (list(s.shape), list(d_y.shape)))
-    norm, held = _describe(torch, d_y, weight, eps, s)
-    # the struct describes d_y with s as residual: for the backward pass what was normalised stands in front
-    (d_y_rows, s_rows, weight_) = held
-    d_y_stride, s_stride = norm.x_stride, norm.residual_stride
-    norm.x, norm.x_stride, norm.residual, norm.residual_stride = s_rows.data_ptr(), s_stride, None, 0
+    numbers, (d_y_rows, d_y_stride), s_rows, dense_weight = _describe(torch, d_y, weight, eps, s)
+    # that describes d_y with s as residual: for the backward pass what was normalised stands in front
+    norm = _norm(numbers, s_rows, (None, 0), dense_weight)
     same = s.dtype == d_y.dtype
-    d_x = torch.empty(s.shape, dtype=d_y.dtype, device=s.device)
-    d_total = d_x if same else (torch.empty(s.shape, dtype=s.dtype, device=s.device) if both else None)
-    d_weight = torch.empty(tuple(weight.shape), dtype=weight.dtype, device=s.device)
+    d_x = _new(torch, d_y)
+    d_total = d_x if same else (_new(torch, s) if both else None)
+    d_weight = _new(torch, weight)
     d_s_rows, d_s_stride = None, 0
     if d_s is not None:
         _check(torch, d_s, 'd_s', s, (s.dtype,))
         if d_s.shape != s.shape:
             raise TypeError('d_s must be %s, got %s' % (list(s.shape), list(d_s.shape)))
         d_s_rows, d_s_stride = _rows(d_s)
-    if norm.rows == 0:
+    if s.numel() == 0:
         return d_x, d_total, d_weight.zero_()
     lib = library()
-    need = lib.ovl_norm_workspace_bytes(ctypes.byref(norm))
+    need = lib.ovl_norm_workspace_bytes(norm)
     work = torch.empty(need, dtype=torch.uint8, device=s.device)
-    with _on(torch, s.device):
-        _call(lib.ovl_norm_backward(ctypes.byref(norm), d_y_rows.data_ptr(), d_y_stride,
+    with _on(torch, s.get_device()):
+        _call(lib.ovl_norm_backward(norm, d_y_rows.data_ptr(), d_y_stride,
                                     None if d_s_rows is None else d_s_rows.data_ptr(), d_s_stride, d_x.data_ptr(),
                                     None if same or d_total is None else d_total.data_ptr(), d_weight.data_ptr(),
-                                    work.data_ptr(), need, torch.cuda.current_stream(s.device).cuda_stream))
+                                    work.data_ptr(), need, torch._C._cuda_getCurrentRawStream(s.get_device())))
     return d_x, d_total, d_weight
 
 

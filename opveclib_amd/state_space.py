@@ -18,8 +18,10 @@ clamped to 0 .. length): returned states are those after the last token, outputs
 what the padding holds is not looked at.
 """
 
+import contextlib
 import ctypes
 import os
+import struct
 import subprocess
 
 from . import local
@@ -102,6 +104,14 @@ class Conv(ctypes.Structure):
                 ('bias', ctypes.c_void_p), ('kept', Sequence), ('lengths', ctypes.c_void_p)]
 
 
+# Packers of the structs above for the calls below: filling a ctypes structure costs ten times as much as packing its
+# fields into a bytes object, and a call for one token has little else to do.
+_pack_scan = struct.Struct('@7I4x22Q').pack
+_pack_conv = struct.Struct('@6I9Q').pack
+_pack_gradients = struct.Struct('@13Q').pack
+_pack_sequence = struct.Struct('@3Q').pack
+
+
 _lib = None
 
 
@@ -160,15 +170,18 @@ def _type_code(dtype):
 
 
 class _Arguments(object):
-    """Checks tensors of one call against its first one, and keeps those it had to copy alive until the launch."""
+    """Checks tensors of one call against its first one, and keeps those it had to copy alive until the launch.  Addresses
+    of tensors that are not there are 0."""
+    __slots__ = ('torch', 'device', 'index', 'dtype', 'code', 'kept')
 
     def __init__(self, torch, first, name):
         self.torch = torch
         if not isinstance(first, torch.Tensor):
             raise TypeError(name + ' must be a torch tensor')
-        if first.device.type != 'cuda':
+        if not first.is_cuda:
             raise RuntimeError('the state space kernels run on an AMD GPU: tensors must live on a HIP device')
         self.device = first.device
+        self.index = first.get_device()
         self.dtype = first.dtype
         self.code = _type_code(first.dtype)
         self.kept = []
@@ -176,48 +189,51 @@ class _Arguments(object):
     def tensor(self, t, name, shape, dtype):
         if not isinstance(t, self.torch.Tensor):
             raise TypeError(name + ' must be a torch tensor')
-        if t.device != self.device:
+        if t.get_device() != self.index:
             raise TypeError('%s is on %s, expected %s' % (name, t.device, self.device))
         if t.dtype != dtype:
             raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise TypeError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
         return t
 
-    def side_by_side(self, t):
-        if (t.stride(-1) != 1 and t.shape[-1] != 1) or (t.dim() > 2 and t.stride(1) > MAX_TOKEN_STRIDE):
-            t = t.contiguous()
-            self.kept.append(t)
-        return t
-
-    def sequence(self, t, name, shape):
-        """[batch, length, channels], or [batch, channels] for one token."""
-        if t is None:
-            return (None, 0, 0)
-        t = self.side_by_side(self.tensor(t, name, shape, self.dtype))
-        strides = t.stride()
-        return (t.data_ptr(), strides[0], strides[1] if len(shape) == 3 else 0)
-
-    def vectors(self, t, name, shape):
-        """[batch, length, groups, state], or without the length for one token; without the groups if there is one."""
-        t = self.side_by_side(self.tensor(t, name, shape, self.dtype))
-        strides = t.stride()
-        return (t.data_ptr(),) + strides[:-1]
-
-    def parameter(self, t, name, shape):
-        """A dense float32 tensor's address, or None."""
-        if t is None:
-            return None
-        t = self.tensor(t, name, shape, self.torch.float32)
+    def dense(self, t):
         if not t.is_contiguous():
             t = t.contiguous()
             self.kept.append(t)
         return t.data_ptr()
 
+    def sequence(self, t, name, shape):
+        """Address and strides of [batch, length, channels], or [batch, channels] for one token."""
+        if t is None:
+            return 0, 0, 0
+        return self.strided(self.tensor(t, name, shape, self.dtype), shape)[:3]
+
+    def vectors(self, t, name, shape, groups):
+        """Address and strides of [batch, length, groups, state], or without the length for one token; without the groups
+        if there is one."""
+        at = self.strided(self.tensor(t, name, shape, self.dtype), shape)
+        return at if groups is None or len(shape) == 4 else (at[0], at[1], 0, at[2])
+
+    def strided(self, t, shape):
+        """(address, the strides but for the last axis, zeros): that axis has stride 1, and tokens are not too far apart."""
+        strides = t.stride()
+        if (strides[-1] != 1 and shape[-1] != 1) or (len(shape) > 2 and strides[1] > MAX_TOKEN_STRIDE):
+            t = t.contiguous()
+            self.kept.append(t)
+            strides = t.stride()
+        return (t.data_ptr(),) + strides[:-1] + (0, 0)[:4 - len(shape)]
+
+    def parameter(self, t, name, shape):
+        """A dense float32 tensor's address."""
+        if t is None:
+            return 0
+        return self.dense(self.tensor(t, name, shape, self.torch.float32))
+
     def weights(self, t, name, shape):
         """A parameter of the convolution: float32, or the sequences' type, which is converted."""
         if t is None:
-            return None
+            return 0
         if not isinstance(t, self.torch.Tensor):
             raise TypeError(name + ' must be a torch tensor')
         if t.dtype == self.dtype and t.dtype != self.torch.float32:
@@ -227,39 +243,39 @@ class _Arguments(object):
 
     def lengths(self, t, batch):
         if t is None:
-            return None
-        t = self.tensor(t, 'lengths', (batch,), self.torch.int32)
-        if not t.is_contiguous():
-            t = t.contiguous()
-            self.kept.append(t)
-        return t.data_ptr()
+            return 0
+        return self.dense(self.tensor(t, 'lengths', (batch,), self.torch.int32))
+
+    def new(self, like):
+        """A dense tensor of that shape and type for a result."""
+        return self.torch.empty_like(like, memory_format=self.torch.contiguous_format)
 
     def scratch(self, nbytes):
-        """Uninitialised device memory of that size: its address, or None for nothing."""
+        """Uninitialised device memory of that size: its address."""
         if nbytes == 0:
-            return None
+            return 0
         t = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
         self.kept.append(t)
         return t.data_ptr()
 
     def stream(self):
-        return self.torch.cuda.current_stream(self.device).cuda_stream
+        return self.torch._C._cuda_getCurrentRawStream(self.index)
+
+    def on(self):
+        """The device of the call as the current one; without the cost of switching where it is already."""
+        return _here if self.index == self.torch.cuda.current_device() else self.torch.cuda.device(self.index)
 
 
-def _on(torch, device):
-    """The device of the call as the current one; without the cost of switching where it is already."""
-    import contextlib
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_here = contextlib.nullcontext()
 
 
 # ----------------------------------------------------------------------------------------------------------------------
 # the scan
 # ----------------------------------------------------------------------------------------------------------------------
 def _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, token=False):
+    """(the checked arguments, ``ovl_ssm_scan`` as bytes, (batch, length, channels, state))"""
     args = _Arguments(torch, u, 'u')
-    shape = tuple(u.shape)
+    shape = u.shape
     if len(shape) != (2 if token else 3):
         raise TypeError('u must be %s, got %s' % ('[batch, channels]' if token else '[batch, length, channels]', list(shape)))
     batch, channels = shape[0], shape[-1]
@@ -271,10 +287,10 @@ def _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, 
     n = A.shape[1]
     if not 1 <= n <= MAX_STATE:
         raise TypeError('A must have 1 to %d state entries per channel, got %d' % (MAX_STATE, n))
-    groups = 1
     if not isinstance(B, torch.Tensor):
         raise TypeError('B must be a torch tensor')
-    lead = shape[:-1]
+    groups = None
+    lead = (batch,) if token else (batch, length)
     if B.dim() == len(lead) + 2:
         groups = B.shape[-2]
         if groups < 1 or channels % groups != 0:
@@ -282,40 +298,31 @@ def _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, 
         vector_shape = lead + (groups, n)
     else:
         vector_shape = lead + (n,)
-    b = args.vectors(B, 'B', vector_shape)
-    c = args.vectors(C, 'C', vector_shape)
-
-    def four(v):
-        v = list(v)
-        if token:
-            v.insert(2, 0)
-        return tuple(v) if len(v) == 4 else tuple(v) + (0,)
-
-    scan = Scan(batch, length, channels, n, groups, args.code, 1 if softplus else 0,
-                args.sequence(u, 'u', shape), args.sequence(delta, 'delta', shape), args.sequence(z, 'z', shape),
-                four(b), four(c),
-                args.parameter(A, 'A', (channels, n)), args.parameter(D, 'D', (channels,)),
-                args.parameter(delta_bias, 'delta_bias', (channels,)),
-                None if token else args.parameter(state, 'state', (batch, channels, n)),
-                args.lengths(lengths, batch))
-    return args, scan, vector_shape
+    b = args.vectors(B, 'B', vector_shape, groups)
+    c = args.vectors(C, 'C', vector_shape, groups)
+    scan_ = _pack_scan(batch, length, channels, n, groups or 1, args.code, 1 if softplus else 0,
+                       *args.sequence(u, 'u', shape), *args.sequence(delta, 'delta', shape), *args.sequence(z, 'z', shape),
+                       *b, *c, args.parameter(A, 'A', (channels, n)), args.parameter(D, 'D', (channels,)),
+                       args.parameter(delta_bias, 'delta_bias', (channels,)),
+                       0 if token else args.parameter(state, 'state', (batch, channels, n)), args.lengths(lengths, batch))
+    return args, scan_, (batch, length, channels, n)
 
 
 def _scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, keep):
     import torch
-    args, scan, _ = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths)
-    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-    last = torch.empty((scan.batch, scan.channels, scan.state), dtype=torch.float32, device=u.device)
-    if y.numel() == 0:
+    args, scan_, (batch, length, channels, n) = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state,
+                                                               lengths)
+    y = args.new(u)
+    last = torch.empty((batch, channels, n), dtype=torch.float32, device=args.device)
+    if batch == 0 or length == 0:
         return y, (last.zero_() if state is None else last.copy_(state.detach())), None
     lib = library()
-    ref = ctypes.byref(scan)
     saved = None
     if keep:
-        saved = torch.empty(lib.ovl_ssm_scan_saved_bytes(ref) // 4, dtype=torch.float32, device=u.device)
-    need = lib.ovl_ssm_scan_workspace_bytes(ref, 0)
-    with _on(torch, args.device):
-        _call(lib.ovl_ssm_scan_forward(ref, y.data_ptr(), last.data_ptr(), None if saved is None else saved.data_ptr(),
+        saved = torch.empty(lib.ovl_ssm_scan_saved_bytes(scan_) // 4, dtype=torch.float32, device=args.device)
+    need = lib.ovl_ssm_scan_workspace_bytes(scan_, 0)
+    with args.on():
+        _call(lib.ovl_ssm_scan_forward(scan_, y.data_ptr(), last.data_ptr(), None if saved is None else saved.data_ptr(),
                                        args.scratch(need), need, args.stream()))
     return y, last, saved
 
@@ -348,44 +355,39 @@ def scan_grad(u, delta, A, B, C, d_y, D=None, z=None, delta_bias=None, softplus=
     :return: (d_u, d_delta, d_A, d_B, d_C, d_D, d_z, d_delta_bias, d_state), None for what was not given
     """
     import torch
-    args, scan_, vector_shape = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths)
-
-    def new(shape, dtype, wanted=True):
-        return torch.empty(shape, dtype=dtype, device=u.device) if wanted else None
-
-    f32 = torch.float32
-    state_shape = (scan_.batch, scan_.channels, scan_.state)
-    d_y_at = args.sequence(d_y, 'd_y', tuple(u.shape))
-    if d_y_at[0] is None:
+    args, scan_, (batch, length, channels, n) = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state,
+                                                               lengths)
+    state_shape = (batch, channels, n)
+    if d_y is None:
         raise TypeError('d_y must be a torch tensor')
-    out = (new(u.shape, u.dtype), new(u.shape, u.dtype), new(A.shape, f32), new(vector_shape, u.dtype),
-           new(vector_shape, u.dtype), new((scan_.channels,), f32, D is not None), new(u.shape, u.dtype, z is not None),
-           new((scan_.channels,), f32, delta_bias is not None), new(state_shape, f32, state is not None))
-    if u.numel() == 0:
+    d_y_at = args.sequence(d_y, 'd_y', u.shape)
+    d_last_at = args.parameter(d_last, 'd_last', state_shape)
+    out = (args.new(u), args.new(u), args.new(A), args.new(B), args.new(B), None if D is None else args.new(D),
+           None if z is None else args.new(u), None if delta_bias is None else args.new(delta_bias),
+           None if state is None else args.new(state))
+    if batch == 0 or length == 0:
         for t in out:
             if t is not None:
                 t.zero_()
         if out[8] is not None and d_last is not None:
-            out[8].copy_(args.tensor(d_last, 'd_last', state_shape, f32).detach())
+            out[8].copy_(d_last.detach())
         return out
-    d_last_at = args.parameter(d_last, 'd_last', state_shape)
-    at = [None if t is None else t.data_ptr() for t in out]
-    gradients = ScanGradients(d_y_at, d_last_at, at[0], at[1], at[6], at[3], at[4], at[2], at[5], at[7], at[8])
+    d_u, d_delta, d_A, d_B, d_C, d_D, d_z, d_bias, d_state = [0 if t is None else t.data_ptr() for t in out]
+    gradients = _pack_gradients(*d_y_at, d_last_at, d_u, d_delta, d_z, d_B, d_C, d_A, d_D, d_bias, d_state)
     lib = library()
-    ref = ctypes.byref(scan_)
-    with _on(torch, args.device):
+    with args.on():
         stream = args.stream()
-        need = lib.ovl_ssm_scan_saved_bytes(ref)
+        need = lib.ovl_ssm_scan_saved_bytes(scan_)
         if saved is None:
-            saved = torch.empty(need // 4, dtype=f32, device=u.device)
-            work = lib.ovl_ssm_scan_workspace_bytes(ref, 0)
-            _call(lib.ovl_ssm_scan_forward(ref, None, None, saved.data_ptr(), args.scratch(work), work, stream))
+            saved = torch.empty(need // 4, dtype=torch.float32, device=args.device)
+            work = lib.ovl_ssm_scan_workspace_bytes(scan_, 0)
+            _call(lib.ovl_ssm_scan_forward(scan_, None, None, saved.data_ptr(), args.scratch(work), work, stream))
         else:
-            args.tensor(saved, 'saved', (need // 4,), f32)
+            args.tensor(saved, 'saved', (need // 4,), torch.float32)
             if not saved.is_contiguous():
                 raise TypeError('saved must be contiguous')
-        work = lib.ovl_ssm_scan_workspace_bytes(ref, 1)
-        _call(lib.ovl_ssm_scan_backward(ref, saved.data_ptr(), ctypes.byref(gradients), args.scratch(work), work, stream))
+        work = lib.ovl_ssm_scan_workspace_bytes(scan_, 1)
+        _call(lib.ovl_ssm_scan_backward(scan_, saved.data_ptr(), gradients, args.scratch(work), work, stream))
     return out
 
 
@@ -398,14 +400,14 @@ def scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, softplu
     :return: y [batch, channels]
     """
     import torch
-    args, scan_, _ = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, None, None, token=True)
-    shape = (scan_.batch, scan_.channels, scan_.state)
-    stride = _in_place(args, state, shape, torch.float32)[0]
-    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-    if y.numel() == 0:
+    args, scan_, (batch, _, channels, n) = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, None, None,
+                                                          token=True)
+    stride = _in_place(args, state, (batch, channels, n), torch.float32)[0]
+    y = args.new(u)
+    if batch == 0:
         return y
-    with _on(torch, args.device):
-        _call(library().ovl_ssm_scan_step(ctypes.byref(scan_), state.data_ptr(), stride, y.data_ptr(), args.stream()))
+    with args.on():
+        _call(library().ovl_ssm_scan_step(scan_, state.data_ptr(), stride, y.data_ptr(), args.stream()))
     return y
 
 
@@ -482,8 +484,9 @@ def _silu(activation):
 
 
 def _describe_conv(torch, x, weight, bias, activation, state, lengths, token=False):
+    """(the checked arguments, ``ovl_ssm_conv`` as bytes, the shape of the state)"""
     args = _Arguments(torch, x, 'x')
-    shape = tuple(x.shape)
+    shape = x.shape
     if len(shape) != (2 if token else 3):
         raise TypeError('x must be %s, got %s' % ('[batch, channels]' if token else '[batch, length, channels]', list(shape)))
     batch, channels = shape[0], shape[-1]
@@ -497,16 +500,14 @@ def _describe_conv(torch, x, weight, bias, activation, state, lengths, token=Fal
     kept_shape = (batch, width - 1, channels)
     if token:
         strides = _in_place(args, state, kept_shape, x.dtype)
-        kept = (state.data_ptr() if width > 1 else None, strides[0], strides[1])
-    elif state is None or width == 1:
-        if state is not None:
-            args.tensor(state, 'state', kept_shape, x.dtype)
-        kept = (None, 0, 0)
+        kept = (state.data_ptr() if width > 1 else 0, strides[0], strides[1])
     else:
         kept = args.sequence(state, 'state', kept_shape)
-    conv_ = Conv(batch, 1 if token else shape[1], channels, width, args.code, _silu(activation),
-                 args.sequence(x, 'x', shape), args.weights(weight, 'weight', (channels, width)),
-                 args.weights(bias, 'bias', (channels,)), kept, args.lengths(lengths, batch))
+        if width == 1:
+            kept = (0, 0, 0)
+    conv_ = _pack_conv(batch, 1 if token else shape[1], channels, width, args.code, _silu(activation),
+                       *args.sequence(x, 'x', shape), args.weights(weight, 'weight', (channels, width)),
+                       args.weights(bias, 'bias', (channels,)), *kept, args.lengths(lengths, batch))
     return args, conv_, kept_shape
 
 
@@ -524,12 +525,12 @@ def conv(x, weight, bias=None, activation=None, state=None, lengths=None):
     """
     import torch
     args, conv_, kept_shape = _describe_conv(torch, x, weight, bias, activation, state, lengths)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    last = torch.empty(kept_shape, dtype=x.dtype, device=x.device)
+    y = args.new(x)
+    last = torch.empty(kept_shape, dtype=x.dtype, device=args.device)
     if y.numel() == 0:
         return y, (last.zero_() if state is None else last.copy_(state.detach()))
-    with _on(torch, args.device):
-        _call(library().ovl_ssm_conv_forward(ctypes.byref(conv_), y.data_ptr(), last.data_ptr(), args.stream()))
+    with args.on():
+        _call(library().ovl_ssm_conv_forward(conv_, y.data_ptr(), last.data_ptr(), args.stream()))
     return y, last
 
 
@@ -541,15 +542,14 @@ def conv_grad(x, weight, d_y, bias=None, activation=None, state=None, lengths=No
     """
     import torch
     args, conv_, kept_shape = _describe_conv(torch, x, weight, bias, activation, state, lengths)
-    f32 = torch.float32
-    d_y_at = args.sequence(d_y, 'd_y', tuple(x.shape))
-    if d_y_at[0] is None:
+    if d_y is None:
         raise TypeError('d_y must be a torch tensor')
+    d_y_at = _pack_sequence(*args.sequence(d_y, 'd_y', x.shape))
     d_last_at = args.sequence(d_last, 'd_last', kept_shape)
-    d_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    d_weight = torch.empty(tuple(weight.shape), dtype=f32, device=x.device)
-    d_bias = None if bias is None else torch.empty((conv_.channels,), dtype=f32, device=x.device)
-    d_state = None if state is None else torch.empty(kept_shape, dtype=x.dtype, device=x.device)
+    d_x = args.new(x)
+    d_weight = torch.empty(weight.shape, dtype=torch.float32, device=args.device)
+    d_bias = None if bias is None else torch.empty(bias.shape, dtype=torch.float32, device=args.device)
+    d_state = None if state is None else args.new(state)
     if x.numel() == 0:
         d_weight.zero_()
         if d_bias is not None:
@@ -558,14 +558,12 @@ def conv_grad(x, weight, d_y, bias=None, activation=None, state=None, lengths=No
             d_state.zero_() if d_last is None else d_state.copy_(d_last.detach())
     else:
         lib = library()
-        ref = ctypes.byref(conv_)
-        need = lib.ovl_ssm_conv_workspace_bytes(ref)
-        d_y_seq, d_last_seq = Sequence(*d_y_at), Sequence(*d_last_at)
-        with _on(torch, args.device):
-            _call(lib.ovl_ssm_conv_backward(ref, ctypes.byref(d_y_seq),
-                                            None if d_last_at[0] is None else ctypes.byref(d_last_seq), d_x.data_ptr(),
-                                            None if d_state is None or conv_.width == 1 else d_state.data_ptr(),
-                                            d_weight.data_ptr(), None if d_bias is None else d_bias.data_ptr(),
+        need = lib.ovl_ssm_conv_workspace_bytes(conv_)
+        with args.on():
+            _call(lib.ovl_ssm_conv_backward(conv_, d_y_at, None if d_last_at[0] == 0 else _pack_sequence(*d_last_at),
+                                            d_x.data_ptr(),
+                                            0 if d_state is None or kept_shape[1] == 0 else d_state.data_ptr(),
+                                            d_weight.data_ptr(), 0 if d_bias is None else d_bias.data_ptr(),
                                             args.scratch(need), need, args.stream()))
     return (d_x, d_weight.to(weight.dtype), None if d_bias is None else d_bias.to(bias.dtype), d_state)
 
@@ -580,11 +578,11 @@ def conv_step(x, state, weight, bias=None, activation=None):
     """
     import torch
     args, conv_, _ = _describe_conv(torch, x, weight, bias, activation, state, None, token=True)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = args.new(x)
     if y.numel() == 0:
         return y
-    with _on(torch, args.device):
-        _call(library().ovl_ssm_conv_step(ctypes.byref(conv_), y.data_ptr(), args.stream()))
+    with args.on():
+        _call(library().ovl_ssm_conv_step(conv_, y.data_ptr(), args.stream()))
     return y
 
 

@@ -78,10 +78,9 @@ def test_long_sequences_are_split_without_a_trace(size, dtype):
     d = ref.scan_inputs(9, batch, length, channels, n, groups, dtype, ragged=batch > 1, device='cuda')
     if batch > 1:
         d['lengths'][0] = 40
-    _, struct, _ = state_space._describe_scan(torch, d['u'], d['delta'], d['A'], d['B'], d['C'], d['D'], d['z'],
+    _, packed, _ = state_space._describe_scan(torch, d['u'], d['delta'], d['A'], d['B'], d['C'], d['D'], d['z'],
                                               d['delta_bias'], True, d['state'], d['lengths'])
-    import ctypes
-    assert state_space.library().ovl_ssm_scan_workspace_bytes(ctypes.byref(struct), 0) > 0
+    assert state_space.library().ovl_ssm_scan_workspace_bytes(packed, 0) > 0
     check_scan(d, terms=32)
 
 

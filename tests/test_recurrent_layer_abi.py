@@ -175,3 +175,23 @@ def test_python_functions_refuse_host_tensors_and_other_things():
         state_space._silu('relu')
     with pytest.raises(ValueError):
         rms_norm.rms_norm_quantized(u, torch.ones(8), group=64)
+
+
+def test_calls_pack_their_structs_as_the_headers_lay_them_out():
+    def same(packed, structure):
+        expected = bytes(structure)
+        assert len(packed) == len(expected) and packed == expected
+
+    numbers = iter(range(1, 100))
+    some = lambda count: [next(numbers) for _ in range(count)]
+    v = some(29)
+    same(state_space._pack_scan(*v), state_space.Scan(*v[:7], *[tuple(v[i:j]) for i, j in ((7, 10), (10, 13), (13, 16), (16, 20), (20, 24))],
+                                                     *v[24:]))
+    v = some(15)
+    same(state_space._pack_conv(*v), state_space.Conv(*v[:6], tuple(v[6:9]), v[9], v[10], tuple(v[11:14]), v[14]))
+    v = some(13)
+    same(state_space._pack_gradients(*v), state_space.ScanGradients(tuple(v[:3]), *v[3:]))
+    v = some(3)
+    same(state_space._pack_sequence(*v), state_space.Sequence(*v))
+    v = some(5) + [0.25] + some(5)
+    same(rms_norm._pack(*v), rms_norm.Norm(*v))
