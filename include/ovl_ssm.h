@@ -102,10 +102,11 @@ typedef struct ovl_ssm_conv {
     int32_t  dtype;                                    /* of x, kept and the sequences written */
     int32_t  silu;
     ovl_ssm_sequence x;
-    const float* weight;                               /* [channels, width] */
-    const float* bias;                                 /* [channels] or NULL */
+    const void* weight;                                /* [channels, width] */
+    const void* bias;                                  /* [channels] or NULL */
     ovl_ssm_sequence kept;                             /* [batch, width - 1, channels]: the tokens before; may be absent */
     const int32_t* lengths;                            /* [batch] or NULL */
+    int32_t  own_weights;                              /* weight and bias are of type dtype; 0: float32 */
 } ovl_ssm_conv;
 
 /* y [batch, length, channels]; last [batch, width - 1, channels]: the tokens a later call needs in `kept`. */

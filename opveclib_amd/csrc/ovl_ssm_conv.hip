@@ -49,7 +49,8 @@ template <typename T> struct conv_args {
     uint32_t batch, length, channels;
     int32_t  silu;
     sequence<T> x, kept;
-    const float *weight, *bias;
+    const void *weight, *bias;
+    bool own_weights;                       // weight and bias are T, else float32
     const int32_t* lengths;
 };
 
@@ -91,63 +92,88 @@ __device__ __forceinline__ void load_line(float (&to)[VEC], const conv_args<T>& 
     }
 }
 
-template <int W, int VEC>
-__device__ __forceinline__ void load_taps(float (&w)[W][VEC], float (&bias)[VEC], const float* weight, const float* b, uint32_t c) {
+// COUNT neighbours at an address that is a multiple of their size only.
+template <typename E, int COUNT> struct __attribute__((packed, aligned(sizeof(E)))) neighbours { E v[COUNT]; };
+
+template <int W, int VEC, typename E>
+__device__ __forceinline__ void load_taps_as(float (&w)[W][VEC], float (&bias)[VEC], const E* weight, const E* b, uint32_t c) {
+    const neighbours<E, VEC * W> taps = *reinterpret_cast<const neighbours<E, VEC * W>*>(weight + (uint64_t)c * W);
+    neighbours<E, VEC> more = {};
+    if (b != nullptr) more = *reinterpret_cast<const neighbours<E, VEC>*>(b + c);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) w[k][i] = weight[(uint64_t)(c + i) * W + k];
-        bias[i] = b != nullptr ? b[c + i] : 0.0f;
+        for (int k = 0; k < W; ++k) w[k][i] = widen<E>(taps.v[i * W + k]);
+        bias[i] = b != nullptr ? widen<E>(more.v[i]) : 0.0f;
     }
 }
 
-// A lane takes RUN tokens of VEC channels; lanes run along the channels first.
-template <typename T, int W, int VEC, int RUN>
+template <typename T, int W, int VEC>
+__device__ __forceinline__ void load_taps(float (&w)[W][VEC], float (&bias)[VEC], const conv_args<T>& p, uint32_t c) {
+    if (p.own_weights)
+        load_taps_as(w, bias, static_cast<const T*>(p.weight), static_cast<const T*>(p.bias), c);
+    else
+        load_taps_as(w, bias, static_cast<const float*>(p.weight), static_cast<const float*>(p.bias), c);
+}
+
+// A lane walks along `slice_tokens` tokens of VEC channels, STEP of them loaded ahead; lanes run along the channels first.
+template <typename T, int W, int VEC>
 __global__ void __launch_bounds__(THREADS)
-conv_forward_kernel(conv_args<T> p, uint32_t vectors, uint32_t runs, T* y, T* last) {
+conv_forward_kernel(conv_args<T> p, uint32_t vectors, uint32_t slices, uint32_t slice_tokens, T* y, T* last) {
+    constexpr uint32_t STEP = 8;
     const uint64_t id = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
-    if (id >= (uint64_t)p.batch * runs * vectors) return;
+    if (id >= (uint64_t)p.batch * slices * vectors) return;
     const uint32_t c = (uint32_t)(id % vectors) * VEC;
     const uint64_t rest = id / vectors;
-    const uint32_t run = (uint32_t)(rest % runs), b = (uint32_t)(rest / runs);
-    const uint32_t t0 = run * RUN, end = end_of(p, b);
-    float w[W][VEC], bias[VEC];
-    load_taps<W, VEC>(w, bias, p.weight, p.bias, c);
-
+    const uint32_t slice = (uint32_t)(rest % slices), b = (uint32_t)(rest / slices);
+    const uint32_t t0 = slice * slice_tokens, end = end_of(p, b), t1 = min(t0 + slice_tokens, p.length), stop = min(t1, end);
+    T* to = y + ((uint64_t)b * p.length + t0) * p.channels + c;
+    uint32_t t = t0;
     if (t0 < end) {
-        // all loads first; tokens behind the sequence are read as its last one and not used
+        float w[W][VEC], bias[VEC], line[W][VEC];           // line: the W inputs of the present token, oldest first
+        load_taps<T>(w, bias, p, c);
         const T* base = p.x.data + (int64_t)b * p.x.batch_stride + c;
-        pack<T, VEC> raw[RUN];
+        pack<T, VEC> next[STEP];
+        // tokens behind the slice are read as its last one and not used
+        auto fetch = [&](uint32_t from) {
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) raw[i] = load_pack<T, VEC>(base + (int64_t)min(t0 + i, end - 1u) * p.x.token_stride);
-        float line[W][VEC];                 // the W inputs of the present token, oldest first
+            for (uint32_t i = 0; i < STEP; ++i)
+                next[i] = load_pack<T, VEC>(base + (int64_t)min(from + i, stop - 1u) * p.x.token_stride);
+        };
+        fetch(t0);
 #pragma unroll
         for (int k = 1; k < W; ++k) load_line<T, W, VEC>(line[k], p, b, c, (int64_t)t0 - W + k);
+        for (; t < stop; t += STEP) {
+            pack<T, VEC> now[STEP];
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-            const uint32_t t = t0 + i;
-            float out[VEC];
+            for (uint32_t i = 0; i < STEP; ++i) now[i] = next[i];
+            if (t + STEP < stop) fetch(t + STEP);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
+            for (uint32_t i = 0; i < STEP; ++i) {
+                float out[VEC];
 #pragma unroll
-                for (int k = 0; k + 1 < W; ++k) line[k][v] = line[k + 1][v];
-                line[W - 1][v] = widen<T>(raw[i].v[v]);
-                float pre = bias[v];
+                for (int v = 0; v < VEC; ++v) {
 #pragma unroll
-                for (int k = 0; k < W; ++k) pre = fmaf(w[k][v], line[k][v], pre);
-                if (p.silu) pre *= sigmoid_(pre);
-                out[v] = t < end ? pre : 0.0f;
+                    for (int k = 0; k + 1 < W; ++k) line[k][v] = line[k + 1][v];
+                    line[W - 1][v] = widen<T>(now[i].v[v]);
+                    float pre = bias[v];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) pre = fmaf(w[k][v], line[k][v], pre);
+                    if (p.silu) pre *= sigmoid_(pre);
+                    out[v] = pre;
+                }
+                if (t + i < stop) store_pack<T, VEC>(to + (uint64_t)i * p.channels, out);
             }
-            if (t < p.length) store_pack<T, VEC>(y + ((uint64_t)b * p.length + t) * p.channels + c, out);
+            to += (uint64_t)STEP * p.channels;
         }
-    } else {
+    }
+    if (stop < t1) {                        // behind the sequence the outputs are zero
         float zero[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) zero[v] = 0.0f;
-        for (uint32_t t = t0; t < min(t0 + RUN, p.length); ++t)
-            store_pack<T, VEC>(y + ((uint64_t)b * p.length + t) * p.channels + c, zero);
+        for (t = max(t0, end); t < t1; ++t) store_pack<T, VEC>(y + ((uint64_t)b * p.length + t) * p.channels + c, zero);
     }
-    if (run == 0u) {
+    if (slice == 0u) {
 #pragma unroll
         for (int k = 0; k + 1 < W; ++k) {
             float row[VEC];
@@ -189,7 +215,7 @@ conv_backward_kernel(conv_args<T> p, conv_gradient_args<T> g, uint32_t vectors, 
         const uint32_t b = (uint32_t)(slice / slices), t0 = (uint32_t)(slice % slices) * slice_tokens;
         const uint32_t end = end_of(p, b), t1 = min(t0 + slice_tokens, p.length);
         float w[W][VEC], bias[VEC], line[W][VEC], d[W][VEC];
-        load_taps<W, VEC>(w, bias, p.weight, p.bias, c);
+        load_taps<T>(w, bias, p, c);
         const T* x_base = p.x.data + (int64_t)b * p.x.batch_stride + c;
         const T* dy_base = g.d_y.data + (int64_t)b * g.d_y.batch_stride + c;
 #pragma unroll
@@ -302,7 +328,7 @@ conv_step_kernel(conv_args<T> p, uint32_t vectors, T* kept, T* y) {
     if (id >= (uint64_t)p.batch * vectors) return;
     const uint32_t c = (uint32_t)(id % vectors) * VEC, b = (uint32_t)(id / vectors);
     float w[W][VEC], bias[VEC];
-    load_taps<W, VEC>(w, bias, p.weight, p.bias, c);
+    load_taps<T>(w, bias, p, c);
     T* own = kept + (int64_t)b * p.kept.batch_stride + c;
     pack<T, VEC> line[W];
 #pragma unroll
@@ -370,29 +396,29 @@ conv_args<T> make_args(const ovl_ssm_conv* s) {
     auto seq = [](const ovl_ssm_sequence& v) {
         return sequence<T>{static_cast<const T*>(v.data), v.batch_stride, v.token_stride};
     };
-    return conv_args<T>{s->batch, s->length, s->channels, s->silu, seq(s->x), seq(s->kept), s->weight, s->bias, s->lengths};
+    return conv_args<T>{s->batch, s->length, s->channels, s->silu, seq(s->x), seq(s->kept), s->weight, s->bias,
+                        s->own_weights != 0, s->lengths};
 }
 
 template <typename T, int W, int VEC>
 void forward(const ovl_ssm_conv* s, T* y, T* last, hipStream_t stream) {
     const uint32_t vectors = s->channels / VEC;
-    // 16 tokens per lane read 1.19 times the input at width 4, 4 tokens 1.75 times: few tokens per lane only where many
-    // would leave compute units without work
-    const bool many = (uint64_t)s->batch * s->length * vectors >= 16ull * 64 * 2048;
-    auto launch = [&](auto kernel, uint32_t run) {
-        const uint32_t runs = (s->length + run - 1) / run;
-        const uint64_t all = (uint64_t)s->batch * runs * vectors;
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)((all + THREADS - 1) / THREADS)), dim3(THREADS), 0, stream, make_args<T>(s),
-                           vectors, runs, y, last);
-    };
-    if (many) launch(conv_forward_kernel<T, W, VEC, 16>, 16u);
-    else launch(conv_forward_kernel<T, W, VEC, 4>, 4u);
+    // so many tokens per lane that the wavefronts fill the compute units once, but at least 4
+    constexpr uint64_t WANTED = 64 * 3072;                  // lanes
+    const uint64_t strands = (uint64_t)s->batch * vectors, most = (s->length + 3u) / 4u;
+    uint64_t slices = WANTED / strands;
+    slices = slices < 1 ? 1 : slices > most ? most : slices;
+    const uint32_t slice_tokens = (uint32_t)((s->length + slices - 1) / slices);
+    slices = (s->length + slice_tokens - 1u) / slice_tokens;
+    const uint64_t all = strands * slices;
+    hipLaunchKernelGGL((conv_forward_kernel<T, W, VEC>), dim3((uint32_t)((all + THREADS - 1) / THREADS)), dim3(THREADS), 0, stream,
+                       make_args<T>(s), vectors, (uint32_t)slices, slice_tokens, y, last);
 }
 
 // How the backward pass cuts the work: a grid of `columns` by `rows` workgroups.
 struct cut { uint32_t vectors, lanes, columns, slices, slice_tokens, rows; };
 cut cut_for(const ovl_ssm_conv* s, uint32_t vec) {
-    constexpr uint64_t WANTED = 2048;       // workgroups
+    constexpr uint64_t WANTED = 512;        // workgroups
     cut k;
     k.vectors = s->channels / vec;
     k.lanes = 64;

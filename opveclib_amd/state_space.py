@@ -101,13 +101,14 @@ class Conv(ctypes.Structure):
     """``ovl_ssm_conv``"""
     _fields_ = [(n, ctypes.c_uint32) for n in ('batch', 'length', 'channels', 'width')] + \
                [('dtype', ctypes.c_int32), ('silu', ctypes.c_int32), ('x', Sequence), ('weight', ctypes.c_void_p),
-                ('bias', ctypes.c_void_p), ('kept', Sequence), ('lengths', ctypes.c_void_p)]
+                ('bias', ctypes.c_void_p), ('kept', Sequence), ('lengths', ctypes.c_void_p),
+                ('own_weights', ctypes.c_int32)]
 
 
 # Packers of the structs above for the calls below: filling a ctypes structure costs ten times as much as packing its
 # fields into a bytes object, and a call for one token has little else to do.
 _pack_scan = struct.Struct('@7I4x22Q').pack
-_pack_conv = struct.Struct('@6I9Q').pack
+_pack_conv = struct.Struct('@6I9QI4x').pack
 _pack_gradients = struct.Struct('@13Q').pack
 _pack_sequence = struct.Struct('@3Q').pack
 
@@ -230,16 +231,19 @@ class _Arguments(object):
             return 0
         return self.dense(self.tensor(t, name, shape, self.torch.float32))
 
-    def weights(self, t, name, shape):
-        """A parameter of the convolution: float32, or the sequences' type, which is converted."""
-        if t is None:
-            return 0
-        if not isinstance(t, self.torch.Tensor):
-            raise TypeError(name + ' must be a torch tensor')
-        if t.dtype == self.dtype and t.dtype != self.torch.float32:
-            t = t.detach().float()
-            self.kept.append(t)
-        return self.parameter(t, name, shape)
+    def weights(self, weight, bias, width, channels):
+        """(address of the taps, of the bias, whether they are of the sequences' type and not float32).  A call that mixes
+        the types has the narrow one converted."""
+        f32 = self.torch.float32
+        own = self.dtype != f32 and weight.dtype == self.dtype and (bias is None or bias.dtype == self.dtype)
+        at = []
+        for t, name, shape in ((weight, 'weight', (channels, width)), (bias, 'bias', (channels,))):
+            if t is not None:
+                if not own and t.dtype == self.dtype != f32:
+                    t = t.detach().to(f32)
+                    self.kept.append(t)
+                at.append(self.dense(self.tensor(t, name, shape, self.dtype if own else f32)))
+        return at[0], at[1] if bias is not None else 0, 1 if own else 0
 
     def lengths(self, t, batch):
         if t is None:
@@ -505,9 +509,11 @@ def _describe_conv(torch, x, weight, bias, activation, state, lengths, token=Fal
         kept = args.sequence(state, 'state', kept_shape)
         if width == 1:
             kept = (0, 0, 0)
+    if bias is not None and not isinstance(bias, torch.Tensor):
+        raise TypeError('bias must be a torch tensor')
+    taps, more, own = args.weights(weight, bias, width, channels)
     conv_ = _pack_conv(batch, 1 if token else shape[1], channels, width, args.code, _silu(activation),
-                       *args.sequence(x, 'x', shape), args.weights(weight, 'weight', (channels, width)),
-                       args.weights(bias, 'bias', (channels,)), *kept, args.lengths(lengths, batch))
+                       *args.sequence(x, 'x', shape), taps, more, *kept, args.lengths(lengths, batch), own)
     return args, conv_, kept_shape
 
 

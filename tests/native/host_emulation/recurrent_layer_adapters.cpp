@@ -64,6 +64,7 @@ extern "C" int emu_recurrent_layer(const ovl_tensor* in, uint32_t n_in, ovl_tens
         p.x = {at(in[1]), s[7], s[8]};
         p.weight = at<float>(in[2]);
         p.bias = at<float>(in[3]);
+        p.own_weights = in[0].len > 9 ? (int32_t)s[9] : 0;
         p.kept = {at(in[4]), rows * p.channels, p.channels};
         p.lengths = at<int32_t>(in[5]);
         if (s[0] == 3) {

@@ -279,6 +279,26 @@ def test_parameters_of_the_sequences_type():
     assert grads[1].dtype == torch.bfloat16 and grads[2].dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize('dtype', ['bfloat16', 'float16'])
+@pytest.mark.parametrize('channels,width', [(16, 4), (12, 3), (7, 4), (600, 2)])
+def test_weights_of_the_sequences_type_are_widened(channels, width, dtype):
+    """Bit for bit the call with the same weights in float32, also where only one of the two is narrow."""
+    kind = ref.TYPES[dtype]
+    d = ref.conv_inputs(22, 2, 33, channels, width, dtype, ragged=True, entering=True, device='cuda')
+    w, b = d['weight'].to(kind), d['bias'].to(kind)
+
+    def all_forms(w, b):
+        y, last = state_space.conv(d['x'], w, b, 'silu', d['state'], d['lengths'])
+        grads = state_space.conv_grad(d['x'], w, d['d_y'], b, 'silu', d['state'], d['lengths'], d['d_last'])
+        own = d['state'].clone()
+        return [y, last, state_space.conv_step(d['x'][:, 0].contiguous(), own, w, b, 'silu'), own] + list(grads)
+
+    want = all_forms(w.float(), b.float())
+    for weight, bias in ((w, b), (w, b.float()), (w.float(), b)):
+        for got, expected in zip(all_forms(weight, bias), want):
+            assert torch.equal(got, expected.to(got.dtype))
+
+
 def test_autograd_functions_give_the_gradients():
     d = ref.scan_inputs(21, 2, 35, 12, 16, 1, 'float32', ragged=True, device='cuda')
     leaves = {k: d[k].clone().requires_grad_(True) for k in ref.SCAN_NAMES}

@@ -187,8 +187,8 @@ def test_calls_pack_their_structs_as_the_headers_lay_them_out():
     v = some(29)
     same(state_space._pack_scan(*v), state_space.Scan(*v[:7], *[tuple(v[i:j]) for i, j in ((7, 10), (10, 13), (13, 16), (16, 20), (20, 24))],
                                                      *v[24:]))
-    v = some(15)
-    same(state_space._pack_conv(*v), state_space.Conv(*v[:6], tuple(v[6:9]), v[9], v[10], tuple(v[11:14]), v[14]))
+    v = some(16)
+    same(state_space._pack_conv(*v), state_space.Conv(*v[:6], tuple(v[6:9]), v[9], v[10], tuple(v[11:14]), *v[14:]))
     v = some(13)
     same(state_space._pack_gradients(*v), state_space.ScanGradients(tuple(v[:3]), *v[3:]))
     v = some(3)

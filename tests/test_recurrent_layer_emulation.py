@@ -192,6 +192,19 @@ def test_conv_step(program, case):
     assert torch.equal(state.double(), want_last)
 
 
+@pytest.mark.parametrize('channels', [16, 7])
+def test_conv_with_weights_of_the_sequences_type(program, channels):
+    d = ref.conv_inputs(6, 2, 5, channels, 4, 'bfloat16')
+    narrow = [d[n].bfloat16() for n in ('weight', 'bias')]
+    results = []
+    for own, (w, b) in enumerate(([t.float() for t in narrow], narrow)):
+        results.append(run(program, [3, 2, 5, channels, 4, ref.CODES['bfloat16'], 1, 5 * channels, channels, own],
+                           [d['x'], w, b, d['state'], None],
+                           [((2, 5, channels), torch.bfloat16), ((2, 3, channels), torch.bfloat16)]))
+    for wide, own in zip(*results):
+        assert torch.equal(wide, own)
+
+
 NORMS = [
     # rows, columns, type, residual's type or None, weight's type
     (1, 1, 'float32', None, 'float32'),
