@@ -34,15 +34,23 @@ template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) pack { 
 
 // Eight columns from `c` on of a row, zero past its end.
 template <typename T>
+__device__ __forceinline__ pack<T> load_raw(const T* row, uint32_t c, uint32_t columns) {
+    if (c + VEC <= columns) return *reinterpret_cast<const pack<T>*>(row + c);
+    pack<T> raw;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) raw.v[i] = c + i < columns ? row[c + i] : narrow<T>(0.0f);
+    return raw;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen_vec(float (&to)[VEC], const pack<T>& raw) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) to[i] = widen<T>(raw.v[i]);
+}
+
+template <typename T>
 __device__ __forceinline__ void load_vec(float (&to)[VEC], const T* row, uint32_t c, uint32_t columns) {
-    if (c + VEC <= columns) {
-        const pack<T> raw = *reinterpret_cast<const pack<T>*>(row + c);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) to[i] = widen<T>(raw.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) to[i] = c + i < columns ? widen<T>(row[c + i]) : 0.0f;
-    }
+    widen_vec<T>(to, load_raw<T>(row, c, columns));
 }
 
 template <typename T>
@@ -156,8 +164,10 @@ norm_forward_kernel(norm_args p, T* y, R* summed, uint8_t* q, float* scales) {
     across<LANES, max_op>(squares, largest, lds);
     const float rstd = ovl_lane::rsq_(fmaf(squares, p.over_columns, p.eps));
     // one scale for the row: max |y| = rstd max |s w|
+    // (a scale below the smallest normal number is taken as that: its reciprocal would not be finite)
+    auto scale_of = [](float top) { return top > 0.0f ? fmaxf(top / E4M3_MAX, 0x1p-126f) : 1.0f; };
     const float row_largest = largest * rstd;
-    if (QUANTIZED && !GROUPED && lane == 0u) scales[row] = row_largest > 0.0f ? row_largest / E4M3_MAX : 1.0f;
+    if (QUANTIZED && !GROUPED && lane == 0u) scales[row] = scale_of(row_largest);
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
         const uint32_t c = (h * LANES + lane) * VEC;
@@ -175,9 +185,9 @@ norm_forward_kernel(norm_args p, T* y, R* summed, uint8_t* q, float* scales) {
                 top = row_all<max_op>(top);
                 const uint32_t group = c / 128u, groups = (p.columns + 127u) / 128u;
                 if ((lane & 15u) == 0u && group < groups)
-                    scales[row * groups + group] = top > 0.0f ? top / E4M3_MAX : 1.0f;
+                    scales[row * groups + group] = scale_of(top);
             }
-            const float inverse = top > 0.0f ? E4M3_MAX / top : 0.0f;
+            const float inverse = top > 0.0f ? fminf(E4M3_MAX / top, 0x1p126f) : 0.0f;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) out[i] *= inverse;
             struct __attribute__((packed, aligned(1))) bytes { uint32_t v[2]; } packed;
@@ -214,22 +224,42 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
     for (int h = 0; h < HELD; ++h)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dw[h][i] = 0.0f;
-    uint32_t turn = 0;
-    for (uint64_t row = team; row < p.rows; row += teams, turn ^= 1u) {
-        const R* x = static_cast<const R*>(p.x) + (int64_t)row * p.x_stride;
+    float w[HELD][VEC];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
+    // a row's inputs are read one row ahead where there are registers for it (8192 rows of 4096 columns, bf16 with float32
+    // sums: 106 us, else 113; with four vectors per lane it costs more than it gives: 2048 rows of 32768 take 424 us, and
+    // 970 with rows ahead)
+    constexpr bool AHEAD = HELD <= 2;
+    struct inputs { pack<R> s[HELD]; pack<T> d_y[HELD]; pack<R> d_summed[HELD]; };
+    auto fetch = [&](inputs& to, uint64_t row) {
+        const R* s = static_cast<const R*>(p.x) + (int64_t)row * p.x_stride;
         const T* d_y = static_cast<const T*>(g.d_y) + (int64_t)row * g.d_y_stride;
-        float n[HELD][VEC], t[HELD][VEC];
+        const R* d_summed = static_cast<const R*>(g.d_summed) + (int64_t)row * g.d_summed_stride;
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
             const uint32_t c = (h * LANES + lane) * VEC;
-            load_vec<R>(n[h], x, c, p.columns);
-            load_vec<T>(t[h], d_y, c, p.columns);
+            to.s[h] = load_raw<R>(s, c, p.columns);
+            to.d_y[h] = load_raw<T>(d_y, c, p.columns);
+            if (g.d_summed != nullptr) to.d_summed[h] = load_raw<R>(d_summed, c, p.columns);
+        }
+    };
+    uint32_t turn = 0;
+    inputs now, next;
+    if (AHEAD) fetch(next, team);
+    for (uint64_t row = team; row < p.rows; row += teams, turn ^= 1u) {
+        if (AHEAD) {
+            now = next;
+            if (row + teams < p.rows) fetch(next, row + teams);
+        } else {
+            fetch(now, row);
         }
         // one exchange for both: rstd comes from the sum of s^2, and mean(t n) = rstd mean(t s)
-        float squares = 0.0f, dot = 0.0f, w[HELD][VEC];
+        float squares = 0.0f, dot = 0.0f, n[HELD][VEC], t[HELD][VEC];
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
-            load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
+            widen_vec<R>(n[h], now.s[h]);
+            widen_vec<T>(t[h], now.d_y[h]);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 squares = fmaf(n[h][i], n[h][i], squares);
@@ -251,7 +281,7 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
             }
             if (g.d_summed != nullptr) {
                 float more[VEC];
-                load_vec<R>(more, static_cast<const R*>(g.d_summed) + (int64_t)row * g.d_summed_stride, c, p.columns);
+                widen_vec<R>(more, now.d_summed[h]);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) out[i] += more[i];
             }
@@ -264,19 +294,24 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
         store_vec<float>(dw[h], g.part + (uint64_t)team * p.columns, (h * LANES + lane) * VEC, p.columns);
 }
 
-// Adds the teams' parts up: 64 columns per workgroup, four wavefronts share the parts, in a fixed order.
+// Adds the teams' parts up: 64 columns per workgroup, sixteen wavefronts share the parts, in a fixed order.
+constexpr uint32_t SHARES = 16;
 template <typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(64 * SHARES)
 norm_sum_kernel(const float* part, uint32_t columns, uint32_t teams, W* d_weight) {
-    __shared__ float lds[4][64];
+    __shared__ float lds[SHARES][64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, c = blockIdx.x * 64u + lane;
     float sum = 0.0f;
     if (c < columns)
 #pragma unroll 8
-        for (uint32_t k = wave; k < teams; k += 4u) sum += part[(uint64_t)k * columns + c];
+        for (uint32_t k = wave; k < teams; k += SHARES) sum += part[(uint64_t)k * columns + c];
     lds[wave][lane] = sum;
     __syncthreads();
-    if (wave == 0u && c < columns) d_weight[c] = narrow<W>((lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]));
+    if (wave == 0u && c < columns) {
+#pragma unroll
+        for (uint32_t i = 1; i < SHARES; ++i) sum += lds[i][lane];
+        d_weight[c] = narrow<W>(sum);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -348,10 +383,11 @@ template <typename F> void by_types(const ovl_norm* p, F&& call) {
 
 template <int LANES> constexpr uint32_t threads_of() { return LANES > 256 ? LANES : 256; }
 
-// Teams of the backward pass: as many as fill the compute units twice; a team's part of the weight gradient is written
-// and read once, so few rows get few teams.
+// Teams of the backward pass: two workgroups per compute unit (of 1024 lanes one); a team's part of the weight gradient
+// is written and read once, so few rows get few teams.  Twice as many: 108 us for 103 at 8192 rows of 4096 columns (bf16
+// with float32 sums), 125 for 112 at 32768 of 1000, but 63 for 71 at 65536 of 512 all in bf16.
 uint32_t teams_for(const ovl_norm* p) {
-    const uint32_t most = p->columns <= 2048u ? 4096u : p->columns <= 8192u ? 1024u : 512u;
+    const uint32_t most = p->columns <= 2048u ? 2048u : p->columns <= 8192u ? 512u : 256u;
     const uint32_t few = (p->rows + 3u) / 4u;
     return few < most ? few : most;
 }
@@ -441,10 +477,10 @@ int ovl_norm_backward(const ovl_norm* p, const void* d_y, int64_t d_y_stride, co
         });
         const dim3 grid((p->columns + 63u) / 64u);
         if (p->weight_dtype == OVL_NORM_FLOAT32)
-            hipLaunchKernelGGL((norm_sum_kernel<float>), grid, dim3(256), 0, stream, static_cast<const float*>(workspace),
+            hipLaunchKernelGGL((norm_sum_kernel<float>), grid, dim3(64 * SHARES), 0, stream, static_cast<const float*>(workspace),
                                p->columns, teams, static_cast<float*>(d_weight));
         else
-            hipLaunchKernelGGL((norm_sum_kernel<T>), grid, dim3(256), 0, stream, static_cast<const float*>(workspace),
+            hipLaunchKernelGGL((norm_sum_kernel<T>), grid, dim3(64 * SHARES), 0, stream, static_cast<const float*>(workspace),
                                p->columns, teams, static_cast<T*>(d_weight));
     });
     return after_launch("ovl_norm_backward");

@@ -111,6 +111,22 @@ def test_rows_of_zeros_and_rows_that_are_not_finite():
     assert bool((rms_norm.rms_norm_quantized(x, w)[0].float().abs().amax(1)[[0, 5]] == 448).all())
 
 
+@pytest.mark.parametrize('group', [None, 128])
+def test_scales_stay_normal_numbers(group):
+    """Results so small that a 448th of them is subnormal, whose reciprocal would not be finite."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(5)
+    x = torch.randn(3, 256, generator=g, device='cuda')
+    x[0, 3] = 0
+    w = torch.full((256,), 2.0 ** -124, device='cuda')
+    q, scales = rms_norm.rms_norm_quantized(x, w, group=group)
+    assert bool((scales == 2.0 ** -126).all()) and q[0, 3].item() == 0
+    exact = ref.norm(x.double(), w.double()) * 2.0 ** 126
+    # as in check_quantized; a result below 2^-126 may come out of float32 arithmetic as zero: up to 1 of the 448 steps
+    off = (q.double() - exact).abs()
+    assert bool(((off <= exact.abs() * (2.0 ** -4 + 2.0 ** -20) + 2.0 ** -10 + 2.0 ** -20) | ((q.float() == 0) & (exact.abs() < 1))).all())
+
+
 def test_autograd_function():
     for kind in KINDS:
         x, r, w, d_y, d_s = inputs(3, (21, 260), *kind)
