@@ -4,22 +4,25 @@
 // a[t] = exp(dt[t] A) and b[t] = dt[t] u[t] B[t]; the output sums over the state entries, y[t] = sum C[t] h[t].  The
 // gradient is the same recurrence from the other end: g[t] = C[t] dy[t] + r[t+1], r[t] = a[t] g[t].
 //
-// Work layout.  A quad of lanes owns one channel, each of its lanes S of the channel's (up to 64) state entries in
-// registers; a wavefront owns 16 channels, a workgroup of four wavefronts 64 neighbouring channels of one group and walks
-// along the tokens in tiles of 16.  What depends on (token, channel) only - the loads, softplus, the gate - is done once
-// for four tokens in the four lanes of the quad and handed round with lane moves that are part of the consuming
-// instruction; the sums over the state entries end in an exchange inside the quad that leaves every lane with its own
-// token.  B and C, which all channels of the workgroup share, go through LDS as float32, one barrier per tile, the next
-// tile's loads in flight.
-//
 // Bound.  Per state entry and token: one multiplication and one exponential (two issue slots) for the decay, one
-// multiplication and two fused multiply-adds: 24 clocks of a SIMD per wavefront, measured; at 16 state entries that is
-// more than what the loads and stores take, so the vector ALU bounds the scan.
+// multiplication and two fused multiply-adds: 24 clocks of a SIMD per 64 entries, measured; at 16 state entries that is
+// more than what the loads and stores take, so the vector ALU bounds the scan, and a SIMD needs two wavefronts or more (one
+// alone issues an instruction in 6.3 clocks, several together one in 4.3).
 //
-// Splitting the length.  A sequence is sequential; few channels leave compute units idle.  Then the tokens are split into
-// chunks: one pass computes every chunk's effect on a zero state (the decay of a chunk needs only the sum of its dt), a
-// small kernel joins the chunks' states, and the full pass starts every chunk from its true state.  The price is a second
+// Splitting the length.  A sequence is sequential; few channels leave SIMDs idle.  Then the tokens are split into chunks:
+// one pass computes every chunk's effect on a zero state (the decay of a chunk needs only the sum of its dt), a small
+// kernel joins the chunks' states, and the full pass starts every chunk from its true state.  The price is a second
 // evaluation of every decay, so the split is made only where it pays (chunks_for below).
+//
+// Work layouts.  Where a lane needs nothing but its channel (the forward pass, and the pass over the gradient's chunks) it
+// holds all entries of the channel's state, up to 64, in registers: a wavefront owns 64 neighbouring channels of one group
+// and a chunk, nothing is summed across lanes, and there is no barrier.  B and C, the same for the whole wavefront, come
+// from the lanes of a row as operands of the consuming instructions and through a part of LDS of its own.  Addresses are
+// scalar with 32 bits per lane.  (With a quad per channel the forward pass of 4 sequences of 2048 tokens, 4096 channels of
+// 16 entries in bf16 took 373 us without a split, now it takes 270 with both passes.)
+// The backward pass holds states and decays of several tokens, and sums over channels: a quad owns a channel and its
+// lanes a quarter of the state each; what depends on (token, channel) only is done once for four tokens in the four lanes
+// and handed round with lane moves; sums over the state end in an exchange that leaves every lane with its own token.
 #include <math.h>
 
 #include "ovl_lane.h"
@@ -534,7 +537,7 @@ scan_forward_kernel(scan_args<T> p, uint32_t units, uint32_t chunks, T* y, float
 // (sequence, channel, state entry) in a row, which it reads before any is overwritten, and `walkers` threads (a power of
 // two) stand behind one another: each makes one step (decay, effect) of its chunks, the states between them are joined
 // through LDS, and each hands its own state on.  So 128 chunks are one trip of 16 walkers, where a thread alone would wait
-// for memory 16 times (2048 channels of 16 entries: 19.6 us, now JOIN_US).  REVERSE: the gradient's recurrence, which
+// for memory 16 times (128 chunks of 2048 channels of 16 entries: 19.6 us alone, 9.5 with 16 walkers).  REVERSE: the gradient's recurrence, which
 // enters chunks from their ends.
 constexpr uint32_t AHEAD = 8, MOST_WALKERS = 16;
 constexpr uint32_t join_ids(uint32_t walkers) { return walkers < 4u ? THREADS / walkers : 64u; }
@@ -713,7 +716,7 @@ scan_gradient_local_kernel(scan_args<T> p, uint32_t units, sequence<T> d_y, floa
 // row every addition halves the number of values a lane holds: afterwards quad i of a row holds entries
 // m + (S / 2) (i & 1) of the first (i < 2) or second set; the rows then trade tokens: row r ends with token r.
 template <int S> struct channel_sums {
-    static constexpr int KEPT = S >= 2 ? S / 2 : 1;
+    static constexpr int KEPT = S / 2;
     float kept[KEPT][4];
     __device__ __forceinline__ void add(const float (&first)[S], const float (&second)[S], int k, uint32_t lane) {
         const bool far = lane & 8u, odd = lane & 4u;
@@ -723,14 +726,10 @@ template <int S> struct channel_sums {
             const float a = first[s] + ovl_lane::row_round<8>(first[s]), b = second[s] + ovl_lane::row_round<8>(second[s]);
             v[s] = far ? b : a;
         }
-        if constexpr (S == 1) {
-            kept[0][k] = v[0] + (odd ? ovl_lane::row_up<4>(v[0]) : ovl_lane::row_down<4>(v[0]));
-        } else {
 #pragma unroll
-            for (int m = 0; m < S / 2; ++m) {
-                const float a = v[m] + ovl_lane::row_down<4>(v[m]), b = v[m + S / 2] + ovl_lane::row_up<4>(v[m + S / 2]);
-                kept[m][k] = odd ? b : a;
-            }
+        for (int m = 0; m < KEPT; ++m) {
+            const float a = v[m] + ovl_lane::row_down<4>(v[m]), b = v[m + KEPT] + ovl_lane::row_up<4>(v[m + KEPT]);
+            kept[m][k] = odd ? b : a;
         }
     }
     // Writes the sums to lds [2][TILE][NP] for the four tokens from `t`.
@@ -744,7 +743,7 @@ template <int S> struct channel_sums {
             ovl_lane::swap_halves(b, d);
             float even = a + c, odd = b + d;
             ovl_lane::swap_rows(even, odd);
-            const uint32_t s = S == 1 ? 0u : m + (S / 2) * (quad & 1u);
+            const uint32_t s = m + KEPT * (quad & 1u);
             lds[((quad >> 1) * TILE + t + row) * NP + q * S + s] = even + odd;
         }
     }
@@ -1002,17 +1001,20 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
     }
 }
 
-// Sums the parts of dB and dC over the blocks of a group, and of dA, dD and d_bias over sequences and chunks.  One thread
-// per result; the order of the additions is fixed.
+// Sums the parts of dB and dC over the blocks of a group, one thread per result, and of dA, dD and d_bias over sequences
+// and chunks, of which there may be thousands: there the sixteen wavefronts of a workgroup share the parts of 64 results
+// that lie side by side.  The order of the additions is fixed.
+constexpr uint32_t SHARES = 16;
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(64 * SHARES)
 scan_gradient_sum_kernel(const float* vector_part, const float* A_part, const float* D_part, const float* bias_part,
                          uint32_t batch, uint32_t length, uint32_t channels, uint32_t state, uint32_t padded,
                          uint32_t groups, uint32_t blocks, uint32_t rows, uint32_t vector_groups,
                          T* d_B, T* d_C, float* d_A, float* d_D, float* d_bias) {
+    __shared__ float lds_sums[SHARES][64];
     const uint64_t per_block = (uint64_t)batch * length * 2u * state;
     if (blockIdx.x < vector_groups) {
-        const uint64_t id = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
+        const uint64_t id = (uint64_t)blockIdx.x * (64u * SHARES) + threadIdx.x;
         if (id >= per_block * groups) return;
         const uint32_t g = (uint32_t)(id / per_block);
         const uint64_t in = id % per_block;
@@ -1026,45 +1028,52 @@ scan_gradient_sum_kernel(const float* vector_part, const float* A_part, const fl
         to[(token * groups + g) * state + (n < state ? n : n - state)] = narrow<T>(sum);
         return;
     }
-    // then state + 2 results per channel: dA, dD, d_bias
-    const uint64_t id = (uint64_t)(blockIdx.x - vector_groups) * THREADS + threadIdx.x;
-    const uint32_t n = (uint32_t)(id % (state + 2u));
-    const uint64_t channel = id / (state + 2u);
-    if (channel >= channels) return;
+    // dA in the order of its parts (state_offset above), then dD, then d_bias
+    const uint32_t lane = threadIdx.x & 63u, share = ovl_lane::wavefront(threadIdx.x / 64u), entries = channels * padded;
+    const uint32_t id = (blockIdx.x - vector_groups) * 64u + lane, channel = id < entries ? id / 4u % channels : (id - entries) % channels;
+    const bool in_A = id < entries, in_D = !in_A && id < entries + channels;
+    const uint32_t n = id / 4u / channels * 4u + id % 4u;       // of dA
+    float* to = in_A ? (n < state ? d_A + (uint64_t)channel * state + n : nullptr)
+                     : in_D ? (d_D != nullptr ? d_D + channel : nullptr)
+                            : (d_bias != nullptr && id < entries + 2u * channels ? d_bias + channel : nullptr);
     float sum = 0.0f;
-    if (n < state) {
+    if (to != nullptr) {
+        const float* from = in_A ? A_part + id : (in_D ? D_part : bias_part) + channel;
+        const uint64_t pace = in_A ? entries : channels;
 #pragma unroll 8
-        for (uint32_t k = 0; k < rows; ++k) sum += A_part[(uint64_t)k * channels * padded + state_offset<1>(n, (uint32_t)channel, channels)];
-        d_A[channel * state + n] = sum;
-    } else if ((n == state ? d_D : d_bias) != nullptr) {
-        const float* from = n == state ? D_part : bias_part;
-#pragma unroll 8
-        for (uint32_t k = 0; k < rows; ++k) sum += from[(uint64_t)k * channels + channel];
-        (n == state ? d_D : d_bias)[channel] = sum;
+        for (uint32_t k = share; k < rows; k += SHARES) sum += from[k * pace];
     }
+    lds_sums[share][lane] = sum;
+    __syncthreads();
+    if (share != 0u || to == nullptr) return;
+#pragma unroll
+    for (uint32_t i = 1; i < SHARES; ++i) sum += lds_sums[i][lane];
+    *to = sum;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // one token
 // ---------------------------------------------------------------------------------------------------------------------
 
-// The recurrence once: a quad per (sequence, channel), as above.  Bound by reading and writing the state.
+// The recurrence once: a quad per (sequence, channel), a workgroup for 64 channels of a sequence.  Bound by reading and
+// writing the state.  WHOLE: a lane's S entries are all there, and accessed as vectors of 16 (S = 2: 8) aligned bytes.
 template <typename T, int S, bool WHOLE>
 __global__ void __launch_bounds__(THREADS)
-scan_step_kernel(scan_args<T> p, float* state, int64_t state_stride, T* y) {
-    const uint64_t id = ((uint64_t)blockIdx.x * THREADS + threadIdx.x) / 4u, every = (uint64_t)p.batch * p.channels;
-    const uint32_t q = threadIdx.x & 3u;
-    const bool active = id < every;
-    const uint32_t b = (uint32_t)((active ? id : every - 1u) / p.channels);
-    const uint32_t channel = (uint32_t)((active ? id : every - 1u) % p.channels);
+scan_step_kernel(scan_args<T> p, uint32_t per_sequence, float* state, int64_t state_stride, T* y) {
+    const uint32_t b = blockIdx.x / per_sequence, q = threadIdx.x & 3u;
+    const uint32_t wanted = (blockIdx.x - b * per_sequence) * BLOCK + threadIdx.x / 4u;
+    const bool active = wanted < p.channels;
+    const uint32_t channel = min(wanted, p.channels - 1u);
     float* own = state + (int64_t)b * state_stride + (uint64_t)channel * p.state;
     const float* A = p.A + (uint64_t)channel * p.state;
-    const T* B = p.B.data + (int64_t)b * p.B.batch_stride + (int64_t)(channel / p.per_group) * p.B.group_stride;
-    const T* C = p.C.data + (int64_t)b * p.C.batch_stride + (int64_t)(channel / p.per_group) * p.C.group_stride;
+    const uint32_t group = channel / p.per_group;
+    const T* B = p.B.data + (int64_t)b * p.B.batch_stride + (int64_t)group * p.B.group_stride;
+    const T* C = p.C.data + (int64_t)b * p.C.batch_stride + (int64_t)group * p.C.group_stride;
     float h[S], A_row[S], B_row[S], C_row[S];
-    if constexpr (WHOLE) {                  // all of 4 S entries, S of them 16-byte aligned or a whole vector
+    if constexpr (WHOLE) {
         typedef float vec __attribute__((ext_vector_type(S >= 4 ? 4 : S)));
         constexpr int PIECES = S >= 4 ? S / 4 : 1, WIDE = S >= 4 ? 4 : S;
+        struct __attribute__((packed, aligned(sizeof(T)))) entries { T v[S]; };
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const vec v = *reinterpret_cast<const vec*>(own + q * S + i * WIDE);
@@ -1072,15 +1081,18 @@ scan_step_kernel(scan_args<T> p, float* state, int64_t state_stride, T* y) {
 #pragma unroll
             for (int k = 0; k < WIDE; ++k) { h[i * WIDE + k] = v[k]; A_row[i * WIDE + k] = a[k]; }
         }
+        const entries b_row = *reinterpret_cast<const entries*>(B + q * S), c_row = *reinterpret_cast<const entries*>(C + q * S);
+#pragma unroll
+        for (int s = 0; s < S; ++s) { B_row[s] = widen<T>(b_row.v[s]); C_row[s] = widen<T>(c_row.v[s]); }
     } else {
         load_entries(h, own, q, p.state);
         load_entries(A_row, A, q, p.state);
-    }
 #pragma unroll
-    for (uint32_t s = 0; s < S; ++s) {
-        const uint32_t at = min(q * S + s, p.state - 1u);
-        B_row[s] = q * S + s < p.state ? widen<T>(B[at]) : 0.0f;
-        C_row[s] = q * S + s < p.state ? widen<T>(C[at]) : 0.0f;
+        for (uint32_t s = 0; s < S; ++s) {
+            const uint32_t at = min(q * S + s, p.state - 1u);
+            B_row[s] = q * S + s < p.state ? widen<T>(B[at]) : 0.0f;
+            C_row[s] = q * S + s < p.state ? widen<T>(C[at]) : 0.0f;
+        }
     }
     const float u = widen<T>(p.u.data[(int64_t)b * p.u.batch_stride + channel]);
     float dt = widen<T>(p.delta.data[(int64_t)b * p.delta.batch_stride + channel]);
@@ -1112,7 +1124,7 @@ scan_step_kernel(scan_args<T> p, float* state, int64_t state_stride, T* y) {
     } else {
         store_entries(h, own, q, p.state);
     }
-    if (q == 0u) y[id] = narrow<T>(sum);
+    if (q == 0u) y[(uint64_t)b * p.channels + channel] = narrow<T>(sum);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1128,26 +1140,29 @@ uint32_t entries_of(uint32_t state) { return state <= 8u ? 2u : state <= 16u ? 4
 
 struct plan {
     uint32_t per_group, blocks, tiles, chunks, chunk_tiles, entries;
-    uint64_t strands;                       // workgroups without a split
+    uint64_t strands;                       // 64 channels of a sequence: a wavefront, in the backward pass a workgroup
 };
 
-// Into how many chunks the length is split.
-void chunks_for(plan& p) {
-    constexpr uint64_t ENOUGH = 1024, WANTED = 4096;
-    constexpr uint32_t SHORTEST = 1;        // tiles per chunk
-    p.chunks = 1;
-    if (p.strands < ENOUGH) {
-        const uint64_t wanted = (WANTED + p.strands - 1) / p.strands;
-        const uint32_t most = p.tiles / SHORTEST;
-        p.chunks = (uint32_t)(wanted < most ? wanted : most);
-        if (p.chunks < 3u) p.chunks = 1;
-    }
+enum class direction { forward, backward, token };
+
+// Into how many chunks the length is split: into so many that every SIMD has four wavefronts of the passes with a channel
+// per lane, where the split pays for its second evaluation of the decays.  4096 channels of 16 entries, bf16:
+//   forward    below 1024 strands (one wavefront per SIMD without a split): 12 sequences of 2048 tokens, 768 strands, take
+//              694 us split and 761 else, 16 sequences 813 split and 768 else
+//   backward   below 512, since a strand is four wavefronts of its main kernel: 4 sequences, 256 strands, take 598 us split
+//              and 735 else, 8 sequences 1139 split and 996 else
+// Fewer than six tiles are not worth two more launches (64 tokens of 64 channels of 8 entries: 21 us split, 17 else), but a
+// chunk may be a single tile (3 sequences of 333 tokens, 650 channels of 8 entries in float32: 20 us, with four tiles 45).
+void chunks_for(plan& p, direction of) {
+    const uint64_t enough = of == direction::backward ? 512 : 1024, wanted = (4096 + p.strands - 1) / p.strands;
+    p.chunks = p.strands < enough && p.tiles >= 6u ? (uint32_t)(wanted < p.tiles ? wanted : p.tiles) : 1u;
     p.chunk_tiles = (p.tiles + p.chunks - 1u) / p.chunks;
     p.chunks = (p.tiles + p.chunk_tiles - 1u) / p.chunk_tiles;
 }
 
-// Checks a scan; `token` for the one-token form.
-int check(const char* who, const ovl_ssm_scan* s, bool token, plan& p) {
+// Checks a scan, and plans it.
+int check(const char* who, const ovl_ssm_scan* s, direction of, plan& p) {
+    const bool token = of == direction::token;
     const std::string name(who);
     if (s == nullptr) return fail(OVL_SSM_EINVAL, name + ": null scan");
     if (s->batch == 0 || s->length == 0 || s->channels == 0 || s->state == 0 || s->groups == 0)
@@ -1171,7 +1186,7 @@ int check(const char* who, const ovl_ssm_scan* s, bool token, plan& p) {
     p.blocks = (p.per_group + BLOCK - 1u) / BLOCK;
     p.tiles = (s->length + TILE - 1u) / TILE;
     p.strands = (uint64_t)s->batch * s->groups * p.blocks;
-    chunks_for(p);
+    chunks_for(p, of);
     // every launch has at most 2^31 - 1 workgroups
     const uint64_t most = (1ull << 31) - 1;
     const uint64_t rows = (uint64_t)s->batch * s->channels;
@@ -1282,9 +1297,9 @@ void backward(const ovl_ssm_scan* s, const plan& p, const float* saved, const ov
     else
         hipLaunchKernelGGL((scan_backward_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
     const uint64_t vector_all = (uint64_t)s->groups * s->batch * s->length * 2u * s->state;
-    const uint32_t vector_groups = (uint32_t)((vector_all + THREADS - 1) / THREADS);
-    const uint32_t rest = (uint32_t)(((uint64_t)s->channels * (s->state + 2u) + THREADS - 1) / THREADS);
-    hipLaunchKernelGGL((scan_gradient_sum_kernel<T>), dim3(vector_groups + rest), dim3(THREADS), 0, stream, to.vector_part,
+    const uint32_t vector_groups = (uint32_t)((vector_all + 64u * SHARES - 1u) / (64u * SHARES));
+    const uint32_t rest = (s->channels * (4u * p.entries + 2u) + 63u) / 64u;
+    hipLaunchKernelGGL((scan_gradient_sum_kernel<T>), dim3(vector_groups + rest), dim3(64u * SHARES), 0, stream, to.vector_part,
                        to.A_part, to.D_part, to.bias_part, s->batch, s->length, s->channels, s->state, 4u * p.entries,
                        s->groups, p.blocks, s->batch * p.chunks, vector_groups, static_cast<T*>(g->d_B),
                        static_cast<T*>(g->d_C), g->d_A, g->d_D, g->d_delta_bias);
@@ -1295,11 +1310,11 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 template <typename T, int S>
 void step(const ovl_ssm_scan* s, const plan& p, float* h, int64_t stride, T* y, hipStream_t stream) {
     const scan_args<T> args = make_args<T>(s, p);
-    const uint64_t lanes = (uint64_t)s->batch * s->channels * 4u;
-    const dim3 grid((uint32_t)((lanes + THREADS - 1) / THREADS));
+    const uint32_t per_sequence = (s->channels + BLOCK - 1u) / BLOCK;
+    const dim3 grid(s->batch * per_sequence);
     const bool whole = s->state == 4u * S && aligned16(h) && aligned16(s->A) && stride % 4 == 0;
-    if (whole) hipLaunchKernelGGL((scan_step_kernel<T, S, true>), grid, dim3(THREADS), 0, stream, args, h, stride, y);
-    else hipLaunchKernelGGL((scan_step_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, h, stride, y);
+    if (whole) hipLaunchKernelGGL((scan_step_kernel<T, S, true>), grid, dim3(THREADS), 0, stream, args, per_sequence, h, stride, y);
+    else hipLaunchKernelGGL((scan_step_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, per_sequence, h, stride, y);
 }
 
 // Calls F<T, S>(...) for the scan's element type and state.
@@ -1317,20 +1332,20 @@ extern "C" {
 
 uint64_t ovl_ssm_scan_workspace_bytes(const ovl_ssm_scan* s, int32_t backward_pass) {
     plan p;
-    if (check("ovl_ssm_scan_workspace_bytes", s, false, p) != OVL_SSM_OK) return 0;
+    if (check("ovl_ssm_scan_workspace_bytes", s, backward_pass != 0 ? direction::backward : direction::forward, p) != OVL_SSM_OK) return 0;
     return lay_out(s, p, backward_pass != 0).all * sizeof(float);
 }
 
 uint64_t ovl_ssm_scan_saved_bytes(const ovl_ssm_scan* s) {
     plan p;
-    if (check("ovl_ssm_scan_saved_bytes", s, false, p) != OVL_SSM_OK) return 0;
+    if (check("ovl_ssm_scan_saved_bytes", s, direction::forward, p) != OVL_SSM_OK) return 0;
     return (uint64_t)s->batch * p.tiles * s->channels * 4u * p.entries * sizeof(float);
 }
 
 int ovl_ssm_scan_forward(const ovl_ssm_scan* s, void* y, float* last, float* saved, void* workspace,
                          uint64_t workspace_bytes, void* hip_stream) {
     plan p;
-    const int rc = check("ovl_ssm_scan_forward", s, false, p);
+    const int rc = check("ovl_ssm_scan_forward", s, direction::forward, p);
     if (rc != OVL_SSM_OK) return rc;
     if ((y == nullptr) != (last == nullptr) || (y == nullptr && saved == nullptr))
         return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_forward: y and last go together; without them saved is needed");
@@ -1350,7 +1365,7 @@ int ovl_ssm_scan_forward(const ovl_ssm_scan* s, void* y, float* last, float* sav
 int ovl_ssm_scan_backward(const ovl_ssm_scan* s, const float* saved, const ovl_ssm_scan_gradients* g, void* workspace,
                           uint64_t workspace_bytes, void* hip_stream) {
     plan p;
-    const int rc = check("ovl_ssm_scan_backward", s, false, p);
+    const int rc = check("ovl_ssm_scan_backward", s, direction::backward, p);
     if (rc != OVL_SSM_OK) return rc;
     if (g == nullptr || saved == nullptr || g->d_y.data == nullptr || g->d_u == nullptr || g->d_delta == nullptr ||
         g->d_B == nullptr || g->d_C == nullptr || g->d_A == nullptr || (s->z.data != nullptr && g->d_z == nullptr))
@@ -1371,7 +1386,7 @@ int ovl_ssm_scan_backward(const ovl_ssm_scan* s, const float* saved, const ovl_s
 
 int ovl_ssm_scan_step(const ovl_ssm_scan* s, float* h, int64_t h_batch_stride, void* y, void* hip_stream) {
     plan p;
-    const int rc = check("ovl_ssm_scan_step", s, true, p);
+    const int rc = check("ovl_ssm_scan_step", s, direction::token, p);
     if (rc != OVL_SSM_OK) return rc;
     if (h == nullptr || y == nullptr) return fail(OVL_SSM_EINVAL, "ovl_ssm_scan_step: null tensor");
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
