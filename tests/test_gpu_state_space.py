@@ -84,6 +84,14 @@ def test_long_sequences_are_split_without_a_trace(size, dtype):
     check_scan(d, terms=32)
 
 
+@pytest.mark.parametrize('size', [(1, 2300, 2, 3, 1), (1, 170, 64 * 400, 2, 1), (2, 100, 64 * 300, 1, 2)], ids=str)
+def test_splits_into_more_chunks_than_are_joined_at_once_and_into_unequal_ones(size):
+    """144 chunks in both directions; 11 tiles in 6 resp. 9 chunks; enough channels for a split in one direction only."""
+    batch, length, channels, n, groups = size
+    d = ref.scan_inputs(10, batch, length, channels, n, groups, 'float32', ragged=batch > 1, device='cuda')
+    check_scan(d, terms=32)
+
+
 def test_slow_decay_over_a_long_sequence_keeps_its_precision():
     """Decays near one: the state is a sum over thousands of tokens."""
     d = ref.scan_inputs(11, 1, 3000, 2, 16, 1, 'float32', gate=False, entering=True, device='cuda')
