@@ -117,41 +117,42 @@ def _rows(t):
     return t.contiguous(), columns
 
 
-def _check(torch, t, name, like, dtypes):
+def _check(torch, t, name, index, dtype, wide):
+    """A tensor of that type, or with ``wide`` of float32."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(name + ' must be a torch tensor')
-    if t.get_device() != like.get_device():
-        raise TypeError('%s is on %s, expected %s' % (name, t.device, like.device))
-    if t.dtype not in dtypes:
-        raise TypeError('%s must be %s, got %s' % (name, ' or '.join(str(d) for d in dtypes), t.dtype))
+    if t.get_device() != index:
+        raise TypeError('%s is on %s, expected cuda:%d' % (name, t.device, index))
+    if t.dtype != dtype and not (wide and t.dtype == torch.float32):
+        raise TypeError('%s must be %s%s, got %s' % (name, dtype, ' or torch.float32' if wide else '', t.dtype))
 
 
-def _describe(torch, x, weight, eps, residual):
+def _describe(torch, x, weight, eps, residual, names=('x', 'residual')):
     """The numbers in front of the addresses in ``ovl_norm``, and (rows, row stride) of x, (rows, row stride) of the
     residual - (None, 0) without one - and the dense weight."""
     if not isinstance(x, torch.Tensor):
-        raise TypeError('x must be a torch tensor')
+        raise TypeError(names[0] + ' must be a torch tensor')
     if not x.is_cuda:
         raise RuntimeError('the norm kernels run on an AMD GPU: tensors must live on a HIP device')
-    code = _type_code(x.dtype, 'x')
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_COLUMNS:
-        raise TypeError('x must have 1 to %d columns, got %s' % (MAX_COLUMNS, list(x.shape)))
-    columns = x.shape[-1]
-    types = (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32)
-    _check(torch, weight, 'weight', x, types)
+    dtype, shape, index = x.dtype, x.shape, x.get_device()
+    code = _type_code(dtype, names[0])
+    if not shape or not 1 <= shape[-1] <= MAX_COLUMNS:
+        raise TypeError('%s must have 1 to %d columns, got %s' % (names[0], MAX_COLUMNS, list(shape)))
+    columns = shape[-1]
+    _check(torch, weight, 'weight', index, dtype, True)
     if weight.shape != (columns,):
         raise TypeError('weight must be [%d], got %s' % (columns, list(weight.shape)))
     other, other_code = (None, 0), code
     if residual is not None:
-        _check(torch, residual, 'residual', x, types)
-        if residual.shape != x.shape:
-            raise TypeError('residual must be %s, got %s' % (list(x.shape), list(residual.shape)))
+        _check(torch, residual, names[1], index, dtype, True)
+        if residual.shape != shape:
+            raise TypeError('%s must be %s, got %s' % (names[1], list(shape), list(residual.shape)))
         other = _rows(residual)
         other_code = _codes[residual.dtype]
-    if x.numel() // columns >= 1 << 32:
-        raise TypeError('x must have fewer than 2^32 rows, got %s' % list(x.shape))
-    numbers = (x.numel() // columns, columns, code, other_code, _codes[weight.dtype], eps)
-    return numbers, _rows(x), other, weight.contiguous()
+    count = x.numel() // columns
+    if count >= 1 << 32:
+        raise TypeError('%s must have fewer than 2^32 rows, got %s' % (names[0], list(shape)))
+    return (count, columns, code, other_code, _codes[weight.dtype], eps), _rows(x), other, weight.contiguous()
 
 
 def _norm(numbers, rows, other, weight):
@@ -206,9 +207,9 @@ def rms_norm_quantized(x, weight, eps=1e-5, residual=None, group=None):
     if group not in (None, GROUP_COLUMNS):
         raise ValueError('group must be None or %d, got %r' % (GROUP_COLUMNS, group))
     held = _describe(torch, x, weight, eps, residual)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
     groups = 1 if group is None else -(-x.shape[-1] // group)
-    scales = torch.empty(x.shape[:-1] + (groups,), dtype=torch.float32, device=x.device)
+    scales = x.new_empty(x.shape[:-1] + (groups,), dtype=torch.float32)
     summed = None if residual is None else _new(torch, residual)
     if x.numel() > 0:
         with _on(torch, x.get_device()):
@@ -229,13 +230,9 @@ def rms_norm_grad(s, weight, d_y, d_s=None, eps=1e-5, both=False):
         tensor where the types are the same, and the second is None without ``both`` where they differ
     """
     import torch
-    if not isinstance(d_y, torch.Tensor) or not isinstance(s, torch.Tensor):
-        raise TypeError('s and d_y must be torch tensors')
-    types = (d_y.dtype,) if d_y.dtype == torch.float32 else (d_y.dtype, torch.float32)
-    _check(torch, s, 's', d_y, types)
-    if d_y.shape != s.shape:
-        raise TypeError('d_y must be %s, got %s' % (list(s.shape), list(d_y.shape)))
-    numbers, (d_y_rows, d_y_stride), s_rows, dense_weight = _describe(torch, d_y, weight, eps, s)
+    if not isinstance(s, torch.Tensor):
+        raise TypeError('s must be a torch tensor')
+    numbers, (d_y_rows, d_y_stride), s_rows, dense_weight = _describe(torch, d_y, weight, eps, s, ('d_y', 's'))
     # that describes d_y with s as residual: for the backward pass what was normalised stands in front
     norm = _norm(numbers, s_rows, (None, 0), dense_weight)
     same = s.dtype == d_y.dtype
@@ -244,7 +241,7 @@ def rms_norm_grad(s, weight, d_y, d_s=None, eps=1e-5, both=False):
     d_weight = _new(torch, weight)
     d_s_rows, d_s_stride = None, 0
     if d_s is not None:
-        _check(torch, d_s, 'd_s', s, (s.dtype,))
+        _check(torch, d_s, 'd_s', s.get_device(), s.dtype, False)
         if d_s.shape != s.shape:
             raise TypeError('d_s must be %s, got %s' % (list(s.shape), list(d_s.shape)))
         d_s_rows, d_s_stride = _rows(d_s)
@@ -252,7 +249,7 @@ def rms_norm_grad(s, weight, d_y, d_s=None, eps=1e-5, both=False):
         return d_x, d_total, d_weight.zero_()
     lib = library()
     need = lib.ovl_norm_workspace_bytes(norm)
-    work = torch.empty(need, dtype=torch.uint8, device=s.device)
+    work = s.new_empty(need, dtype=torch.uint8)
     with _on(torch, s.get_device()):
         _call(lib.ovl_norm_backward(norm, d_y_rows.data_ptr(), d_y_stride,
                                     None if d_s_rows is None else d_s_rows.data_ptr(), d_s_stride, d_x.data_ptr(),

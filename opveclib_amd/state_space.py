@@ -173,68 +173,82 @@ def _type_code(dtype):
 class _Arguments(object):
     """Checks tensors of one call against its first one, and keeps those it had to copy alive until the launch.  Addresses
     of tensors that are not there are 0."""
-    __slots__ = ('torch', 'device', 'index', 'dtype', 'code', 'kept')
+    __slots__ = ('torch', 'Tensor', 'f32', 'index', 'dtype', 'code', 'kept')
 
     def __init__(self, torch, first, name):
         self.torch = torch
+        self.Tensor = torch.Tensor
+        self.f32 = torch.float32
         if not isinstance(first, torch.Tensor):
             raise TypeError(name + ' must be a torch tensor')
         if not first.is_cuda:
             raise RuntimeError('the state space kernels run on an AMD GPU: tensors must live on a HIP device')
-        self.device = first.device
         self.index = first.get_device()
         self.dtype = first.dtype
         self.code = _type_code(first.dtype)
         self.kept = []
 
     def tensor(self, t, name, shape, dtype):
-        if not isinstance(t, self.torch.Tensor):
+        if not isinstance(t, self.Tensor):
             raise TypeError(name + ' must be a torch tensor')
         if t.get_device() != self.index:
-            raise TypeError('%s is on %s, expected %s' % (name, t.device, self.device))
+            raise TypeError('%s is on %s, expected cuda:%d' % (name, t.device, self.index))
         if t.dtype != dtype:
             raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
         if t.shape != shape:
             raise TypeError('%s must be %s, got %s' % (name, list(shape), list(t.shape)))
         return t
 
+    def copied(self, t):
+        t = t.contiguous()
+        self.kept.append(t)
+        return t
+
     def dense(self, t):
         if not t.is_contiguous():
-            t = t.contiguous()
-            self.kept.append(t)
+            t = self.copied(t)
         return t.data_ptr()
 
     def sequence(self, t, name, shape):
-        """Address and strides of [batch, length, channels], or [batch, channels] for one token."""
+        """Address and strides of [batch, length, channels], or [batch, channels] for one token: channels side by side,
+        tokens not too far apart."""
         if t is None:
             return 0, 0, 0
-        return self.strided(self.tensor(t, name, shape, self.dtype), shape)[:3]
+        self.tensor(t, name, shape, self.dtype)
+        strides = t.stride()
+        if len(strides) == 2:
+            if strides[1] != 1 and shape[1] != 1:
+                t = self.copied(t)
+                strides = t.stride()
+            return t.data_ptr(), strides[0], 0
+        if (strides[2] != 1 and shape[2] != 1) or strides[1] > MAX_TOKEN_STRIDE:
+            t = self.copied(t)
+            strides = t.stride()
+        return t.data_ptr(), strides[0], strides[1]
 
-    def vectors(self, t, name, shape, groups):
+    def vectors(self, t, name, shape, token, grouped):
         """Address and strides of [batch, length, groups, state], or without the length for one token; without the groups
         if there is one."""
-        at = self.strided(self.tensor(t, name, shape, self.dtype), shape)
-        return at if groups is None or len(shape) == 4 else (at[0], at[1], 0, at[2])
-
-    def strided(self, t, shape):
-        """(address, the strides but for the last axis, zeros): that axis has stride 1, and tokens are not too far apart."""
+        self.tensor(t, name, shape, self.dtype)
         strides = t.stride()
-        if (strides[-1] != 1 and shape[-1] != 1) or (len(shape) > 2 and strides[1] > MAX_TOKEN_STRIDE):
-            t = t.contiguous()
-            self.kept.append(t)
+        if (strides[-1] != 1 and shape[-1] != 1) or (not token and strides[1] > MAX_TOKEN_STRIDE):
+            t = self.copied(t)
             strides = t.stride()
-        return (t.data_ptr(),) + strides[:-1] + (0, 0)[:4 - len(shape)]
+        return t.data_ptr(), strides[0], 0 if token else strides[1], strides[-2] if grouped else 0
 
     def parameter(self, t, name, shape):
         """A dense float32 tensor's address."""
         if t is None:
             return 0
-        return self.dense(self.tensor(t, name, shape, self.torch.float32))
+        self.tensor(t, name, shape, self.f32)
+        if not t.is_contiguous():
+            t = self.copied(t)
+        return t.data_ptr()
 
     def weights(self, weight, bias, width, channels):
         """(address of the taps, of the bias, whether they are of the sequences' type and not float32).  A call that mixes
         the types has the narrow one converted."""
-        f32 = self.torch.float32
+        f32 = self.f32
         own = self.dtype != f32 and weight.dtype == self.dtype and (bias is None or bias.dtype == self.dtype)
         at = []
         for t, name, shape in ((weight, 'weight', (channels, width)), (bias, 'bias', (channels,))):
@@ -254,11 +268,11 @@ class _Arguments(object):
         """A dense tensor of that shape and type for a result."""
         return self.torch.empty_like(like, memory_format=self.torch.contiguous_format)
 
-    def scratch(self, nbytes):
+    def scratch(self, like, nbytes):
         """Uninitialised device memory of that size: its address."""
         if nbytes == 0:
             return 0
-        t = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
+        t = like.new_empty(nbytes, dtype=self.torch.uint8)
         self.kept.append(t)
         return t.data_ptr()
 
@@ -293,20 +307,18 @@ def _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, 
         raise TypeError('A must have 1 to %d state entries per channel, got %d' % (MAX_STATE, n))
     if not isinstance(B, torch.Tensor):
         raise TypeError('B must be a torch tensor')
-    groups = None
-    lead = (batch,) if token else (batch, length)
-    if B.dim() == len(lead) + 2:
+    groups, grouped = 1, B.dim() == len(shape) + 1
+    if grouped:
         groups = B.shape[-2]
         if groups < 1 or channels % groups != 0:
             raise TypeError('the groups of B and C must divide the %d channels, got %d' % (channels, groups))
-        vector_shape = lead + (groups, n)
+        vector_shape = (batch, groups, n) if token else (batch, length, groups, n)
     else:
-        vector_shape = lead + (n,)
-    b = args.vectors(B, 'B', vector_shape, groups)
-    c = args.vectors(C, 'C', vector_shape, groups)
-    scan_ = _pack_scan(batch, length, channels, n, groups or 1, args.code, 1 if softplus else 0,
+        vector_shape = (batch, n) if token else (batch, length, n)
+    scan_ = _pack_scan(batch, length, channels, n, groups, args.code, 1 if softplus else 0,
                        *args.sequence(u, 'u', shape), *args.sequence(delta, 'delta', shape), *args.sequence(z, 'z', shape),
-                       *b, *c, args.parameter(A, 'A', (channels, n)), args.parameter(D, 'D', (channels,)),
+                       *args.vectors(B, 'B', vector_shape, token, grouped),
+                       *args.vectors(C, 'C', vector_shape, token, grouped), args.parameter(A, 'A', (channels, n)), args.parameter(D, 'D', (channels,)),
                        args.parameter(delta_bias, 'delta_bias', (channels,)),
                        0 if token else args.parameter(state, 'state', (batch, channels, n)), args.lengths(lengths, batch))
     return args, scan_, (batch, length, channels, n)
@@ -317,17 +329,17 @@ def _scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, keep):
     args, scan_, (batch, length, channels, n) = _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state,
                                                                lengths)
     y = args.new(u)
-    last = torch.empty((batch, channels, n), dtype=torch.float32, device=args.device)
+    last = u.new_empty((batch, channels, n), dtype=torch.float32)
     if batch == 0 or length == 0:
         return y, (last.zero_() if state is None else last.copy_(state.detach())), None
     lib = library()
     saved = None
     if keep:
-        saved = torch.empty(lib.ovl_ssm_scan_saved_bytes(scan_) // 4, dtype=torch.float32, device=args.device)
+        saved = u.new_empty(lib.ovl_ssm_scan_saved_bytes(scan_) // 4, dtype=torch.float32)
     need = lib.ovl_ssm_scan_workspace_bytes(scan_, 0)
     with args.on():
         _call(lib.ovl_ssm_scan_forward(scan_, y.data_ptr(), last.data_ptr(), None if saved is None else saved.data_ptr(),
-                                       args.scratch(need), need, args.stream()))
+                                       args.scratch(u, need), need, args.stream()))
     return y, last, saved
 
 
@@ -383,15 +395,15 @@ def scan_grad(u, delta, A, B, C, d_y, D=None, z=None, delta_bias=None, softplus=
         stream = args.stream()
         need = lib.ovl_ssm_scan_saved_bytes(scan_)
         if saved is None:
-            saved = torch.empty(need // 4, dtype=torch.float32, device=args.device)
+            saved = u.new_empty(need // 4, dtype=torch.float32)
             work = lib.ovl_ssm_scan_workspace_bytes(scan_, 0)
-            _call(lib.ovl_ssm_scan_forward(scan_, None, None, saved.data_ptr(), args.scratch(work), work, stream))
+            _call(lib.ovl_ssm_scan_forward(scan_, None, None, saved.data_ptr(), args.scratch(u, work), work, stream))
         else:
             args.tensor(saved, 'saved', (need // 4,), torch.float32)
             if not saved.is_contiguous():
                 raise TypeError('saved must be contiguous')
         work = lib.ovl_ssm_scan_workspace_bytes(scan_, 1)
-        _call(lib.ovl_ssm_scan_backward(scan_, saved.data_ptr(), gradients, args.scratch(work), work, stream))
+        _call(lib.ovl_ssm_scan_backward(scan_, saved.data_ptr(), gradients, args.scratch(u, work), work, stream))
     return out
 
 
@@ -532,7 +544,7 @@ def conv(x, weight, bias=None, activation=None, state=None, lengths=None):
     import torch
     args, conv_, kept_shape = _describe_conv(torch, x, weight, bias, activation, state, lengths)
     y = args.new(x)
-    last = torch.empty(kept_shape, dtype=x.dtype, device=args.device)
+    last = x.new_empty(kept_shape)
     if y.numel() == 0:
         return y, (last.zero_() if state is None else last.copy_(state.detach()))
     with args.on():
@@ -553,8 +565,8 @@ def conv_grad(x, weight, d_y, bias=None, activation=None, state=None, lengths=No
     d_y_at = _pack_sequence(*args.sequence(d_y, 'd_y', x.shape))
     d_last_at = args.sequence(d_last, 'd_last', kept_shape)
     d_x = args.new(x)
-    d_weight = torch.empty(weight.shape, dtype=torch.float32, device=args.device)
-    d_bias = None if bias is None else torch.empty(bias.shape, dtype=torch.float32, device=args.device)
+    d_weight = x.new_empty(weight.shape, dtype=torch.float32)
+    d_bias = None if bias is None else x.new_empty(bias.shape, dtype=torch.float32)
     d_state = None if state is None else args.new(state)
     if x.numel() == 0:
         d_weight.zero_()
@@ -570,7 +582,7 @@ def conv_grad(x, weight, d_y, bias=None, activation=None, state=None, lengths=No
                                             d_x.data_ptr(),
                                             0 if d_state is None or kept_shape[1] == 0 else d_state.data_ptr(),
                                             d_weight.data_ptr(), 0 if d_bias is None else d_bias.data_ptr(),
-                                            args.scratch(need), need, args.stream()))
+                                            args.scratch(x, need), need, args.stream()))
     return (d_x, d_weight.to(weight.dtype), None if d_bias is None else d_bias.to(bias.dtype), d_state)
 
 
