@@ -21,10 +21,9 @@
  *
  * Conventions: tensor memory belongs to the caller and must be device accessible; sequences have their channels side by
  * side, batch and token strides (in elements) are free, but for the scan's token strides, which are 0 to 2^25; outputs are
- * dense.  All sums, states and gradients of
- * parameters are float32; only what is stored in the tensors' type is rounded, once.  The functions enqueue kernels on
- * `hip_stream`, return without synchronising, allocate nothing (scratch memory is handed in, its size is asked for
- * first) and give the same bits for the same call.  They return an ovl_status (ovl_launch.h): OVL_EINVAL for arguments
+ * dense.  All sums, states and gradients of parameters are float32; only what is stored in the tensors' type is rounded,
+ * once.  The functions enqueue kernels on `hip_stream`, return without synchronising, allocate nothing (scratch memory is
+ * handed in, its size is asked for first) and give the same bits for the same call.  They return an ovl_status (ovl_launch.h): OVL_EINVAL for arguments
  * they refuse, OVL_EHIP for a HIP error (text from ovl_ssm_last_error).
  */
 #ifndef OVL_SSM_H_

@@ -456,6 +456,7 @@ def _differentiable(name):
             y, last, saved = _scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths,
                                    any(ctx.needs_input_grad))
             ctx.softplus = softplus
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, state, lengths, saved)
             return y, last
 
@@ -463,6 +464,8 @@ def _differentiable(name):
         @once
         def backward(ctx, d_y, d_last):
             u, delta, A, B, C, D, z, delta_bias, state, lengths, saved = ctx.saved_tensors
+            if d_y is None:
+                d_y = torch.zeros_like(u)
             grads = scan_grad(u, delta, A, B, C, d_y, D, z, delta_bias, ctx.softplus, state, lengths, d_last, saved)
             return grads + (None, None)
 
@@ -470,6 +473,7 @@ def _differentiable(name):
         @staticmethod
         def forward(ctx, x, weight, bias, state, lengths, activation):
             ctx.activation = activation
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(x, weight, bias, state, lengths)
             return conv(x, weight, bias, activation, state, lengths)
 
@@ -477,6 +481,8 @@ def _differentiable(name):
         @once
         def backward(ctx, d_y, d_last):
             x, weight, bias, state, lengths = ctx.saved_tensors
+            if d_y is None:
+                d_y = torch.zeros_like(x)
             grads = conv_grad(x, weight, d_y, bias, ctx.activation, state, lengths, d_last)
             return grads + (None, None)
 

@@ -336,6 +336,26 @@ def test_autograd_functions_give_the_gradients():
     close(grad, full.double().sum(1, keepdim=True), F32, 'broadcast', 16)
 
 
+def test_gradients_of_one_output_alone():
+    d = ref.scan_inputs(30, 2, 21, 12, 16, 1, 'float32', device='cuda')
+    c = ref.conv_inputs(30, 2, 21, 12, 4, 'float32', device='cuda')
+    for op, names in (('scan', ref.SCAN_NAMES), ('conv', ref.CONV_NAMES)):
+        v = d if op == 'scan' else c
+        leaves = {k: v[k].clone().requires_grad_(True) for k in names}
+        if op == 'scan':
+            out = state_space.scan_torch(*[leaves[k] for k in ('u', 'delta', 'A', 'B', 'C')], softplus=True,
+                                         **{k: leaves[k] for k in ('D', 'z', 'delta_bias', 'state')})
+            grad = lambda d_y, d_last: run_grad(dict(v, d_y=d_y, d_last=d_last))
+        else:
+            out = state_space.conv_torch(leaves['x'], leaves['weight'], leaves['bias'], 'silu', leaves['state'])
+            grad = lambda d_y, d_last: state_space.conv_grad(c['x'], c['weight'], d_y, c['bias'], 'silu', c['state'], None, d_last)
+        zero_y, zero_last = torch.zeros_like(v['d_y']), torch.zeros_like(v['d_last'])
+        for which, want in ((0, grad(v['d_y'], zero_last)), (1, grad(zero_y, v['d_last']))):
+            got = torch.autograd.grad(out[which], list(leaves.values()), v['d_last' if which else 'd_y'], retain_graph=True)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
 def test_sequences_without_tokens_and_batches_without_sequences():
     for batch, length in ((2, 0), (0, 5)):
         d = ref.scan_inputs(23, batch, length, 6, 4, 1, 'float32', device='cuda')

@@ -64,7 +64,8 @@ def test_scan_entry_points_refuse(libraries):
                           ({'groups': 3}, b'divide'), ({'dtype': 3}, b'element type'), ({'u': empty}, b'null'),
                           ({'delta': empty}, b'null'), ({'B': state_space.Vectors()}, b'null'),
                           ({'C': state_space.Vectors()}, b'null'), ({'A': None}, b'null'),
-                          ({'length': (1 << 30) + 1}, b'2^30'), ({'batch': 1 << 30, 'channels': 1 << 20}, b'too many')):
+                          ({'length': (1 << 30) + 1}, b'2^30'), ({'batch': 1 << 30, 'channels': 1 << 20}, b'too many'),
+                          ({'batch': 1 << 28, 'length': 1 << 30, 'state': 64}, b'too many')):
         s = scan_struct(**changes)
         ref = ctypes.byref(s)
         assert lib.ovl_ssm_scan_forward(ref, P, P, None, None, 0, None) == EINVAL, changes
@@ -107,7 +108,7 @@ def test_conv_entry_points_refuse(libraries):
 
     for changes in ({'batch': 0}, {'length': 0}, {'channels': 0}, {'width': 0}, {'width': 5}, {'dtype': 9},
                     {'x': state_space.Sequence()}, {'weight': None}, {'length': (1 << 30) + 1},
-                    {'batch': 1 << 31, 'channels': 1 << 31}):
+                    {'batch': 1 << 31, 'channels': 1 << 31}, {'batch': 1, 'length': 1, 'channels': (1 << 31) + 8}):
         ref = ctypes.byref(struct(**changes))
         assert lib.ovl_ssm_conv_forward(ref, P, P, None) == EINVAL, changes
         assert lib.ovl_ssm_conv_workspace_bytes(ref) == 0
