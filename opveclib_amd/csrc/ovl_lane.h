@@ -10,6 +10,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+// A kernel that is to keep at least n wavefronts on a SIMD: 512 / n registers for each lane.
+#define OVL_LANE_WAVES(n) __attribute__((amdgpu_waves_per_eu(n)))
+
 namespace ovl_lane {
 
 typedef _Float16 f16;

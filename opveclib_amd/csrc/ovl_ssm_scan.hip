@@ -167,20 +167,20 @@ template <typename T, uint32_t N, uint32_t PACE> struct writer {
     template <int DIRECTION> __device__ __forceinline__ void move() { tile += DIRECTION * (int64_t)(N * PACE) * token_bytes; }
 };
 
-// The elements of a tile of B or C that this thread takes to LDS: TOKENS tokens of NP entries.
+// The elements of a tile of B or C that this thread takes to LDS: TOKENS tokens of NP entries, from entry `first` on.
 template <typename T, uint32_t NP, uint32_t TOKENS, uint32_t LANES> struct vector_stage {
     static constexpr uint32_t ALL = TOKENS * NP, PER = (ALL + LANES - 1) / LANES;
     const T* tile;
     uint32_t token_bytes, own[PER];
     uint32_t lane;
     T raw[PER];
-    __device__ __forceinline__ vector_stage(const vectors<T>& v, const place& w, uint32_t lane_, uint32_t t0, uint32_t n)
+    __device__ __forceinline__ vector_stage(const vectors<T>& v, const place& w, uint32_t lane_, uint32_t t0, uint32_t n, uint32_t first = 0u)
         : tile(v.data + (int64_t)w.b * v.batch_stride + (int64_t)w.g * v.group_stride + (int64_t)t0 * v.token_stride),
           token_bytes((uint32_t)v.token_stride * (uint32_t)sizeof(T)), lane(lane_) {
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i) {
             const uint32_t at = (lane + i * LANES) % ALL;
-            own[i] = at / NP * token_bytes + min(at % NP, n - 1u) * (uint32_t)sizeof(T);
+            own[i] = at / NP * token_bytes + min(first + at % NP, n - 1u) * (uint32_t)sizeof(T);
         }
     }
     __device__ __forceinline__ void load() {
@@ -196,8 +196,8 @@ template <typename T, uint32_t NP, uint32_t TOKENS, uint32_t LANES> struct vecto
             raw[i] = r.template load<T>(own[i] - (token < left ? 0u : (token - left + 1u) * token_bytes), 0u);
         }
     }
-    // Entries past the state and tokens behind the sequence (`tokens` of the tile's are in it) become zero: they then add
-    // nothing anywhere.
+    // Entries past the state (`n` from the first on are in it) and tokens behind the sequence (`tokens` of the tile's are in
+    // it) become zero: they then add nothing anywhere.
     __device__ __forceinline__ void store(float* lds, uint32_t tokens, uint32_t n) const {
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i) {
@@ -618,6 +618,7 @@ template <typename T> struct gradient_args {
     float* d_entering;
     // parts that a later kernel sums: dB and dC per block of channels, dA, dD and d_bias per sequence and chunk
     float *vector_part, *A_part, *D_part, *bias_part;
+    uint32_t padded, slices;                // entries of a state as it is kept; slices of it that are worked on in turn
 };
 
 // The effect of a chunk on a zero gradient entering at its end: r = a (C dy + r), tokens walked from the last.  Lanes as in
@@ -760,26 +761,41 @@ template <int S> struct channel_sums {
 // Bound by the vector ALU: 26 instructions per token and 64 entries (14 of the recurrences, 4.5 of the sums over channels,
 // 2 of the states computed twice, the rest per token and channel), and the vector ALU is busy for 380 of the 490 us that
 // 4 sequences of 2048 tokens, 4096 channels of 16 entries in bf16 take.
-template <typename T, int S, bool GATE>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, int S, bool GATE, bool SLICED>
+__global__ void __launch_bounds__(THREADS) OVL_LANE_WAVES(2)
 scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, const float* entry) {
-    constexpr uint32_t NP = 4 * S;
+    constexpr uint32_t NP = 4 * S, MOST_SLICES = SLICED ? 4 : 1;
     // tokens whose states and decays are held in registers at a time
-    constexpr uint32_t SUB = S <= 2 ? 16 : S <= 4 ? 8 : 4, SUBS = TILE / SUB;
-    __shared__ __attribute__((aligned(16))) float lds_B[2][TILE * NP];
-    __shared__ __attribute__((aligned(16))) float lds_C[2][TILE * NP];
+    constexpr uint32_t SUB = S <= 2 ? 16 : 8, SUBS = TILE / SUB;
+    __shared__ __attribute__((aligned(16))) float lds_B[TILE * NP];
+    __shared__ __attribute__((aligned(16))) float lds_C[TILE * NP];
     __shared__ float lds_sums[WAVES][2 * TILE * NP];
+    // what a lane keeps of the slices it is not working on: r and dA; of a tile's slices before: y and its gradients
+    __shared__ float lds_r[MOST_SLICES][S][SLICED ? THREADS : 1], lds_dA[MOST_SLICES][S][SLICED ? THREADS : 1];
+    __shared__ float lds_before[3][QUADS][SLICED ? THREADS : 1];
     const place w = find_place<4>(p, blockIdx.x, threadIdx.x, 0u, p.chunks);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u, slices = SLICED ? g.slices : 1u;
+    const uint32_t padded = SLICED ? g.padded : NP;
     const uint64_t chunk_row = ((uint64_t)w.b * p.chunks + w.chunk) * p.channels;
     const uint64_t state_row = (uint64_t)w.b * p.channels + w.channel;
+    const float* A_row = p.A + (uint64_t)w.channel * p.state;
 
     float r[S], A2[S], dA[S];
-    load_entries(A2, p.A + (uint64_t)w.channel * p.state, w.q, p.state);
+    auto load_A2 = [&](uint32_t slice) {
+        load_entries(A2, A_row, slice * 4u + w.q, p.state);
 #pragma unroll
-    for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; r[s] = 0.0f; dA[s] = 0.0f; }
-    if (entry != nullptr) load_states(r, entry + chunk_row * NP, w.q * S, w.channel, p.channels);
-    else if (g.d_last != nullptr) load_entries(r, g.d_last + state_row * p.state, w.q, p.state);
+        for (int s = 0; s < S; ++s) A2[s] *= LOG2E;
+    };
+    for (uint32_t slice = 0; slice < slices; ++slice) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) { r[s] = 0.0f; dA[s] = 0.0f; }
+        if (entry != nullptr) load_states(r, entry + chunk_row * padded, (slice * 4u + w.q) * S, w.channel, p.channels);
+        else if (g.d_last != nullptr) load_entries(r, g.d_last + state_row * p.state, slice * 4u + w.q, p.state);
+        if (SLICED)
+#pragma unroll
+            for (int s = 0; s < S; ++s) { lds_r[slice][s][threadIdx.x] = r[s]; lds_dA[slice][s][threadIdx.x] = 0.0f; }
+    }
+    if (!SLICED) load_A2(0u);
     const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
     const float skip = p.D != nullptr ? p.D[w.channel] : 0.0f;
     float dD = 0.0f, dbias = 0.0f;
@@ -790,35 +806,8 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
     typedef vector_stage<T, NP, TILE, THREADS> stage;
     reads u_from(p.u, w, start), delta_from(p.delta, w, start), z_from(p.z, w, start), dy_from(g.d_y, w, start);
     writes out_at(w, p.length, p.channels, start);
-    stage B_next(p.B, w, threadIdx.x, start, p.state), C_next(p.C, w, threadIdx.x, start, p.state);
-    const float* kept = saved + ((uint64_t)w.b * p.tiles + start / TILE) * p.channels * NP;
-    T u_next[QUADS], delta_next[QUADS], z_next[QUADS], dy_next[QUADS];
-    float h_next[S];
-    auto fetch = [&](uint32_t left) {
-        if (left >= TILE) {
-            u_from.load(u_next);
-            delta_from.load(delta_next);
-            dy_from.load(dy_next);
-            if (GATE) z_from.load(z_next);
-            B_next.load();
-            C_next.load();
-        } else {
-            u_from.load_some(u_next, left, w.q);
-            delta_from.load_some(delta_next, left, w.q);
-            dy_from.load_some(dy_next, left, w.q);
-            if (GATE) z_from.load_some(z_next, left, w.q);
-            B_next.load_some(left);
-            C_next.load_some(left);
-        }
-        load_states(h_next, kept, w.q * S, w.channel, p.channels);
-        u_from.template move<-1>();
-        delta_from.template move<-1>();
-        dy_from.template move<-1>();
-        z_from.template move<-1>();
-        B_next.template move<-1>();
-        C_next.template move<-1>();
-        kept -= (uint64_t)p.channels * NP;
-    };
+    stage B_all(p.B, w, threadIdx.x, start, p.state), C_all(p.C, w, threadIdx.x, start, p.state);
+    const float* kept = saved + ((uint64_t)w.b * p.tiles + start / TILE) * p.channels * padded;
     float* const part = g.vector_part + (((uint64_t)w.g * p.blocks + w.block) * p.batch + w.b) * p.length * (2u * p.state);
 
     // behind the sequence all gradients are zero
@@ -834,27 +823,49 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
     }
 
     for (uint32_t tile = stop; tile-- > w.first;) {
-        const uint32_t t0 = tile * TILE, buffer = tile & 1u, left = p.length - t0, tokens = w.end - t0;
-        T du_done[QUADS], ddelta_done[QUADS], dz_done[QUADS];
+        const uint32_t t0 = tile * TILE, left = p.length - t0, tokens = w.end - t0;
+        T u_raw[QUADS], delta_raw[QUADS], z_raw[QUADS], dy_raw[QUADS], du_done[QUADS], ddelta_done[QUADS], dz_done[QUADS];
+        float h_first[S];
+        auto fetch_slice = [&](uint32_t slice, stage& B_stage, stage& C_stage) {
+            if (left >= TILE) {
+                B_stage.load();
+                C_stage.load();
+            } else {
+                B_stage.load_some(left);
+                C_stage.load_some(left);
+            }
+            load_states(h_first, kept, (slice * 4u + w.q) * S, w.channel, p.channels);
+        };
         // Loaded here and not a tile ahead: the registers for that cost the second wavefront of a SIMD, which hides more
         // (261 registers and one wavefront: 690 us, 247 and two: 500 us for 4 x 2048 tokens of 4096 channels).
-        fetch(left);
-        B_next.store(lds_B[buffer], tokens, p.state);
-        C_next.store(lds_C[buffer], tokens, p.state);
-        float u[QUADS], dt[QUADS], x[QUADS], d[QUADS], h[SUBS][S];
+        if (left >= TILE) {
+            u_from.load(u_raw);
+            delta_from.load(delta_raw);
+            dy_from.load(dy_raw);
+            if (GATE) z_from.load(z_raw);
+        } else {
+            u_from.load_some(u_raw, left, w.q);
+            delta_from.load_some(delta_raw, left, w.q);
+            dy_from.load_some(dy_raw, left, w.q);
+            if (GATE) z_from.load_some(z_raw, left, w.q);
+        }
+        if (!SLICED) {
+            fetch_slice(0u, B_all, C_all);
+            B_all.store(lds_B, tokens, p.state);
+            C_all.store(lds_C, tokens, p.state);
+        }
+        float u[QUADS], dt[QUADS], x[QUADS], d[QUADS];
         float slope[QUADS], gate_slope[QUADS];              // d dt / d delta; d z is gate_slope times y
 #pragma unroll
         for (uint32_t j = 0; j < QUADS; ++j) {
             // lanes without a channel of their own add nothing to any sum
-            u[j] = w.active ? widen<T>(u_next[j]) : 0.0f;
-            dt[j] = widen<T>(delta_next[j]) + bias;
-            d[j] = w.active ? widen<T>(dy_next[j]) : 0.0f;
-            gate_slope[j] = GATE ? widen<T>(z_next[j]) : 0.0f;
+            u[j] = w.active ? widen<T>(u_raw[j]) : 0.0f;
+            dt[j] = widen<T>(delta_raw[j]) + bias;
+            d[j] = w.active ? widen<T>(dy_raw[j]) : 0.0f;
+            gate_slope[j] = GATE ? widen<T>(z_raw[j]) : 0.0f;
         }
-#pragma unroll
-        for (int s = 0; s < S; ++s) h[0][s] = h_next[s];
         // also lets every wavefront finish reading lds_sums of the tile before
-        __syncthreads();
+        if (!SLICED) __syncthreads();
         if (tokens < TILE)
 #pragma unroll
             for (uint32_t j = 0; j < QUADS; ++j) {
@@ -886,124 +897,173 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
             dD = fmaf(d[j], u[j], dD);
         }
 
-        // the states that enter the later parts of the tile
+        for (uint32_t slice = 0; slice < slices; ++slice) {
+            const uint32_t first = slice * NP;
+            if (SLICED) {
+                stage B_stage(p.B, w, threadIdx.x, t0, p.state, first), C_stage(p.C, w, threadIdx.x, t0, p.state, first);
+                fetch_slice(slice, B_stage, C_stage);
+                load_A2(slice);
+                B_stage.store(lds_B, tokens, p.state - first);
+                C_stage.store(lds_C, tokens, p.state - first);
 #pragma unroll
-        for (uint32_t part_of = 0; part_of + 1u < SUBS; ++part_of) {
-#pragma unroll
-            for (int s = 0; s < S; ++s) h[part_of + 1u][s] = h[part_of][s];
-#pragma unroll
-            for (uint32_t i = 0; i < SUB; ++i) {
-                const uint32_t at = part_of * SUB + i;
-                const float* Bt = lds_B[buffer] + at * NP + w.q * S;
-                const float dt_k = quad_pick(dt[at / 4u], at & 3u), x_k = quad_pick(x[at / 4u], at & 3u);
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-                    h[part_of + 1u][s] = fmaf(ovl_lane::exp2_(dt_k * A2[s]), h[part_of + 1u][s], x_k * Bt[s]);
-                if (at % 4u == 3u) __builtin_amdgcn_sched_barrier(0);
+                for (int s = 0; s < S; ++s) { r[s] = lds_r[slice][s][threadIdx.x]; dA[s] = lds_dA[slice][s][threadIdx.x]; }
+                // also lets every wavefront finish reading lds_sums of the slice before
+                __syncthreads();
             }
-        }
+            float h[SUBS][S];
+#pragma unroll
+            for (int s = 0; s < S; ++s) h[0][s] = h_first[s];
+            // the states that enter the later parts of the tile
+#pragma unroll
+            for (uint32_t part_of = 0; part_of + 1u < SUBS; ++part_of) {
+#pragma unroll
+                for (int s = 0; s < S; ++s) h[part_of + 1u][s] = h[part_of][s];
+#pragma unroll
+                for (uint32_t i = 0; i < SUB; ++i) {
+                    const uint32_t at = part_of * SUB + i;
+                    const float* Bt = lds_B + at * NP + w.q * S;
+                    const float dt_k = quad_pick(dt[at / 4u], at & 3u), x_k = quad_pick(x[at / 4u], at & 3u);
+#pragma unroll
+                    for (int s = 0; s < S; ++s)
+                        h[part_of + 1u][s] = fmaf(ovl_lane::exp2_(dt_k * A2[s]), h[part_of + 1u][s], x_k * Bt[s]);
+                    if (at % 4u == 3u) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
 
-        float dA_tile[S];
+            float dA_tile[S];
 #pragma unroll
-        for (int s = 0; s < S; ++s) dA_tile[s] = 0.0f;
+            for (int s = 0; s < S; ++s) dA_tile[s] = 0.0f;
 #pragma unroll
-        for (uint32_t back = 0; back < SUBS; ++back) {
-            const uint32_t part_of = SUBS - 1u - back;
-            float a[SUB][S], state[SUB + 1u][S], y[SUB / 4u];
+            for (uint32_t back = 0; back < SUBS; ++back) {
+                const uint32_t part_of = SUBS - 1u - back;
+                float a[SUB][S], state[SUB + 1u][S], y[SUB / 4u];
 #pragma unroll
-            for (int s = 0; s < S; ++s) state[0][s] = h[part_of][s];
+                for (int s = 0; s < S; ++s) state[0][s] = h[part_of][s];
 #pragma unroll
-            for (uint32_t i = 0; i < SUB; i += 4u) {
-                const uint32_t j = part_of * (SUB / 4u) + i / 4u;
-                float sums[4];
+                for (uint32_t i = 0; i < SUB; i += 4u) {
+                    const uint32_t j = part_of * (SUB / 4u) + i / 4u;
+                    float sums[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float* Bt = lds_B[buffer] + (4u * j + k) * NP + w.q * S;
-                    const float* Ct = lds_C[buffer] + (4u * j + k) * NP + w.q * S;
-                    const float dt_k = quad_pick(dt[j], k), x_k = quad_pick(x[j], k);
-                    sums[k] = 0.0f;
+                    for (int k = 0; k < 4; ++k) {
+                        const float* Bt = lds_B + (4u * j + k) * NP + w.q * S;
+                        const float* Ct = lds_C + (4u * j + k) * NP + w.q * S;
+                        const float dt_k = quad_pick(dt[j], k), x_k = quad_pick(x[j], k);
+                        sums[k] = 0.0f;
 #pragma unroll
-                    for (int s = 0; s < S; ++s) {
-                        a[i + k][s] = ovl_lane::exp2_(dt_k * A2[s]);
-                        state[i + k + 1][s] = fmaf(a[i + k][s], state[i + k][s], x_k * Bt[s]);
-                        if (GATE) sums[k] = fmaf(Ct[s], state[i + k + 1][s], sums[k]);
+                        for (int s = 0; s < S; ++s) {
+                            a[i + k][s] = ovl_lane::exp2_(dt_k * A2[s]);
+                            state[i + k + 1][s] = fmaf(a[i + k][s], state[i + k][s], x_k * Bt[s]);
+                            if (GATE) sums[k] = fmaf(Ct[s], state[i + k + 1][s], sums[k]);
+                        }
                     }
+                    y[i / 4u] = GATE ? quad_scatter_sum(sums, w.q) : 0.0f;
+                    // (keeps the scheduler from loading B and C of all tokens at once)
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                y[i / 4u] = GATE ? fmaf(skip, u[j], quad_scatter_sum(sums, w.q)) : 0.0f;
-                // (keeps the scheduler from loading B and C of all tokens at once)
-                __builtin_amdgcn_sched_barrier(0);
-            }
 #pragma unroll
-            for (uint32_t step = 0; step < SUB; step += 4u) {
-                const uint32_t i = SUB - 4u - step, j = part_of * (SUB / 4u) + i / 4u;
-                channel_sums<S> sums;
-                float dx[4], through[4];
+                for (uint32_t step = 0; step < SUB; step += 4u) {
+                    const uint32_t i = SUB - 4u - step, j = part_of * (SUB / 4u) + i / 4u;
+                    channel_sums<S> sums;
+                    float dx[4], through[4];
 #pragma unroll
-                for (int k = 3; k >= 0; --k) {
-                    const float* Bt = lds_B[buffer] + (4u * j + k) * NP + w.q * S;
-                    const float* Ct = lds_C[buffer] + (4u * j + k) * NP + w.q * S;
-                    const float dt_k = quad_pick(dt[j], k), x_k = quad_pick(x[j], k), d_k = quad_pick(d[j], k);
-                    float dB[S], dC[S];
-                    dx[k] = 0.0f;
-                    through[k] = 0.0f;
+                    for (int k = 3; k >= 0; --k) {
+                        const float* Bt = lds_B + (4u * j + k) * NP + w.q * S;
+                        const float* Ct = lds_C + (4u * j + k) * NP + w.q * S;
+                        const float dt_k = quad_pick(dt[j], k), x_k = quad_pick(x[j], k), d_k = quad_pick(d[j], k);
+                        float dB[S], dC[S];
+                        dx[k] = 0.0f;
+                        through[k] = 0.0f;
 #pragma unroll
-                    for (int s = 0; s < S; ++s) {
-                        const float grad = fmaf(d_k, Ct[s], r[s]);
-                        dx[k] = fmaf(grad, Bt[s], dx[k]);
-                        dB[s] = grad * x_k;
-                        dC[s] = d_k * state[i + k + 1][s];
-                        r[s] = grad * a[i + k][s];
-                        const float moved = r[s] * state[i + k][s];
-                        dA_tile[s] = fmaf(dt_k, moved, dA_tile[s]);
-                        through[k] = fmaf(moved, A2[s], through[k]);
+                        for (int s = 0; s < S; ++s) {
+                            const float grad = fmaf(d_k, Ct[s], r[s]);
+                            dx[k] = fmaf(grad, Bt[s], dx[k]);
+                            dB[s] = grad * x_k;
+                            dC[s] = d_k * state[i + k + 1][s];
+                            r[s] = grad * a[i + k][s];
+                            const float moved = r[s] * state[i + k][s];
+                            dA_tile[s] = fmaf(dt_k, moved, dA_tile[s]);
+                            through[k] = fmaf(moved, A2[s], through[k]);
+                        }
+                        sums.add(dB, dC, k, lane);
                     }
-                    sums.add(dB, dC, k, lane);
+                    sums.put(lds_sums[wave], 4u * j, lane);
+                    float d_x = quad_scatter_sum(dx, w.q), d_through = quad_scatter_sum(through, w.q), out = y[i / 4u];
+                    if (SLICED && slice > 0u) {
+                        d_x += lds_before[0][j][threadIdx.x];
+                        d_through += lds_before[1][j][threadIdx.x];
+                        if (GATE) out += lds_before[2][j][threadIdx.x];
+                    }
+                    if (SLICED && slice + 1u < slices) {
+                        lds_before[0][j][threadIdx.x] = d_x;
+                        lds_before[1][j][threadIdx.x] = d_through;
+                        if (GATE) lds_before[2][j][threadIdx.x] = out;
+                    } else {
+                        float d_dt = fmaf(d_x, u[j], LN2 * d_through) * slope[j];
+                        if (tokens < TILE) d_dt = 4u * j + w.q < tokens ? d_dt : 0.0f;
+                        dbias += d_dt;
+                        du_done[j] = narrow<T>(fmaf(d_x, dt[j], skip * d[j]));
+                        ddelta_done[j] = narrow<T>(d_dt);
+                        if (GATE) dz_done[j] = narrow<T>(gate_slope[j] * fmaf(skip, u[j], out));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                sums.put(lds_sums[wave], 4u * j, lane);
-                const float d_x = quad_scatter_sum(dx, w.q);
-                float d_dt = fmaf(d_x, u[j], LN2 * quad_scatter_sum(through, w.q)) * slope[j];
-                if (tokens < TILE) d_dt = 4u * j + w.q < tokens ? d_dt : 0.0f;
-                dbias += d_dt;
-                du_done[j] = narrow<T>(fmaf(d_x, dt[j], skip * d[j]));
-                ddelta_done[j] = narrow<T>(d_dt);
-                if (GATE) dz_done[j] = narrow<T>(gate_slope[j] * y[i / 4u]);
-                __builtin_amdgcn_sched_barrier(0);
             }
-        }
-        if (tokens < TILE)
 #pragma unroll
-            for (uint32_t j = 0; j < QUADS; ++j) {
-                du_done[j] = 4u * j + w.q < tokens ? du_done[j] : narrow<T>(0.0f);
-                if (GATE) dz_done[j] = 4u * j + w.q < tokens ? dz_done[j] : narrow<T>(0.0f);
+            for (int s = 0; s < S; ++s) dA[s] += dA_tile[s];
+            if (SLICED)
+#pragma unroll
+                for (int s = 0; s < S; ++s) { lds_r[slice][s][threadIdx.x] = r[s]; lds_dA[slice][s][threadIdx.x] = dA[s]; }
+
+            // the four wavefronts' sums, as [token][B entries, C entries]
+            auto sum_up = [&] {
+                __syncthreads();
+                for (uint32_t at = threadIdx.x; at < 2u * TILE * NP; at += THREADS) {
+                    const uint32_t set = at / (TILE * NP), t = at / NP % TILE, n = first + at % NP;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (uint32_t v = 0; v < WAVES; ++v) sum += lds_sums[v][at];
+                    if (n < p.state && t < left) part[(uint64_t)(t0 + t) * 2u * p.state + set * p.state + n] = t < tokens ? sum : 0.0f;
+                }
+            };
+            if (SLICED && slice + 1u < slices) {
+                sum_up();
+                continue;
             }
-        if (!w.active) {
-        } else if (left >= TILE) {
-            out_at.store(g.d_u, du_done);
-            out_at.store(g.d_delta, ddelta_done);
-            if (GATE) out_at.store(g.d_z, dz_done);
-        } else {
-            out_at.store_some(g.d_u, du_done, left, w.q);
-            out_at.store_some(g.d_delta, ddelta_done, left, w.q);
-            if (GATE) out_at.store_some(g.d_z, dz_done, left, w.q);
+            if (tokens < TILE)
+#pragma unroll
+                for (uint32_t j = 0; j < QUADS; ++j) {
+                    du_done[j] = 4u * j + w.q < tokens ? du_done[j] : narrow<T>(0.0f);
+                    if (GATE) dz_done[j] = 4u * j + w.q < tokens ? dz_done[j] : narrow<T>(0.0f);
+                }
+            if (!w.active) {
+            } else if (left >= TILE) {
+                out_at.store(g.d_u, du_done);
+                out_at.store(g.d_delta, ddelta_done);
+                if (GATE) out_at.store(g.d_z, dz_done);
+            } else {
+                out_at.store_some(g.d_u, du_done, left, w.q);
+                out_at.store_some(g.d_delta, ddelta_done, left, w.q);
+                if (GATE) out_at.store_some(g.d_z, dz_done, left, w.q);
+            }
+            sum_up();
         }
+        u_from.template move<-1>();
+        delta_from.template move<-1>();
+        dy_from.template move<-1>();
+        z_from.template move<-1>();
+        B_all.template move<-1>();
+        C_all.template move<-1>();
         out_at.template move<-1>();
+        kept -= (uint64_t)p.channels * padded;
+    }
+    if (w.active)
+        for (uint32_t slice = 0; slice < slices; ++slice) {
+            if (SLICED)
 #pragma unroll
-        for (int s = 0; s < S; ++s) dA[s] += dA_tile[s];
-
-        // the four wavefronts' sums, as [token][B entries, C entries]
-        __syncthreads();
-        for (uint32_t at = threadIdx.x; at < 2u * TILE * NP; at += THREADS) {
-            const uint32_t set = at / (TILE * NP), t = at / NP % TILE, n = at % NP;
-            float sum = 0.0f;
-#pragma unroll
-            for (uint32_t v = 0; v < WAVES; ++v) sum += lds_sums[v][at];
-            if (n < p.state && t < left) part[(uint64_t)(t0 + t) * 2u * p.state + set * p.state + n] = t < tokens ? sum : 0.0f;
+                for (int s = 0; s < S; ++s) { r[s] = lds_r[slice][s][threadIdx.x]; dA[s] = lds_dA[slice][s][threadIdx.x]; }
+            store_states(dA, g.A_part + chunk_row * padded, (slice * 4u + w.q) * S, w.channel, p.channels);
+            if (w.chunk == 0u && g.d_entering != nullptr) store_entries(r, g.d_entering + state_row * p.state, slice * 4u + w.q, p.state);
         }
-    }
-    if (w.active) {
-        store_states(dA, g.A_part + chunk_row * NP, w.q * S, w.channel, p.channels);
-        if (w.chunk == 0u && g.d_entering != nullptr) store_entries(r, g.d_entering + state_row * p.state, w.q, p.state);
-    }
     dD = quad_sum(dD);
     dbias = quad_sum(dbias);
     if (w.active && w.q == 0u) {
@@ -1304,10 +1364,14 @@ void backward(const ovl_ssm_scan* s, const plan& p, const float* saved, const ov
         entry = local;
     }
     const dim3 grid((uint32_t)(p.strands * p.chunks));
+    constexpr bool SLICED = S > 4;
+    constexpr int HELD = SLICED ? 4 : S;
+    to.padded = 4u * p.entries;
+    to.slices = (s->state + 4u * HELD - 1u) / (4u * HELD);
     if (s->z.data != nullptr)
-        hipLaunchKernelGGL((scan_backward_kernel<T, S, true>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
+        hipLaunchKernelGGL((scan_backward_kernel<T, HELD, true, SLICED>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
     else
-        hipLaunchKernelGGL((scan_backward_kernel<T, S, false>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
+        hipLaunchKernelGGL((scan_backward_kernel<T, HELD, false, SLICED>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
     const uint64_t vector_all = (uint64_t)s->groups * s->batch * s->length * 2u * s->state;
     const uint32_t vector_groups = (uint32_t)((vector_all + 64u * SHARES - 1u) / (64u * SHARES));
     const uint32_t rest = (s->channels * (4u * p.entries + 2u) + 63u) / 64u;

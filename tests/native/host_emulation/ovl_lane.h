@@ -9,6 +9,8 @@
 static inline uint32_t min(uint32_t a, uint32_t b) { return a < b ? a : b; }
 static inline uint32_t max(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
+#define OVL_LANE_WAVES(n)
+
 namespace ovl_lane {
 
 struct bf16 { uint16_t bits; };
