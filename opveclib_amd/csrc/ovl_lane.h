@@ -40,7 +40,7 @@ __device__ __forceinline__ float rsq_(float x) { return __builtin_amdgcn_rsqf(x)
 __device__ __forceinline__ float positive(float x) { return __builtin_amdgcn_fmed3f(x, 0.0f, __builtin_inff()); }
 
 // The value is in a register at this point of the program: its computation does not move behind it.
-__device__ __forceinline__ void keep(float& x) { asm volatile("" : "+v"(x)); }
+template <typename X> __device__ __forceinline__ void keep(X& x) { asm volatile("" : "+v"(x)); }
 // A number that the whole wavefront shares, as one of which the compiler knows nothing more: what is made of it is made here
 // and not kept from earlier.
 __device__ __forceinline__ uint32_t anew(uint32_t x) {

@@ -228,13 +228,15 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
     for (int h = 0; h < HELD; ++h)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dw[h][i] = 0.0f;
-    float w[HELD][VEC];
-#pragma unroll
-    for (int h = 0; h < HELD; ++h) load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
     // a row's inputs are read one row ahead where there are registers for it (8192 rows of 4096 columns, bf16 with float32
-    // sums: 106 us, else 113; with four vectors per lane it costs more than it gives: 2048 rows of 32768 take 424 us, and
-    // 970 with rows ahead)
-    constexpr bool AHEAD = HELD <= 2;
+    // sums: 106 us, else 113).  A team of 1024 lanes has 128 registers for each and does not read ahead (4096 rows of 16384:
+    // 208 us, 342 with rows ahead in scratch memory); with four vectors per lane it reads a row twice, the second time from
+    // the L2, and holds nothing of it in between (2048 rows of 32768: 284 us, 424 held in scratch memory).
+    constexpr bool AHEAD = HELD <= 2 && LANES <= 256, LEAN = HELD > 2 && LANES > 256;
+    float w[HELD][VEC];
+    if (!LEAN)
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
     struct inputs { pack<R> s[HELD]; pack<T> d_y[HELD]; pack<R> d_summed[HELD]; };
     auto fetch = [&](inputs& to, uint64_t row) {
         const R* s = static_cast<const R*>(p.x) + (int64_t)row * p.x_stride;
@@ -245,8 +247,16 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
             const uint32_t c = (h * LANES + lane) * VEC;
             to.s[h] = load_raw<R>(s, c, p.columns);
             to.d_y[h] = load_raw<T>(d_y, c, p.columns);
-            if (g.d_summed != nullptr) to.d_summed[h] = load_raw<R>(d_summed, c, p.columns);
+            if (!LEAN && g.d_summed != nullptr) to.d_summed[h] = load_raw<R>(d_summed, c, p.columns);
         }
+    };
+    float n[HELD][VEC], t[HELD][VEC];
+    auto again = [&](int h, uint64_t row) {
+        uint32_t c = (h * LANES + lane) * VEC;
+        ovl_lane::keep(c);                  // else the addresses of all its vectors are kept over the rows, in scratch memory
+        load_vec<R>(n[h], static_cast<const R*>(p.x) + (int64_t)row * p.x_stride, c, p.columns);
+        load_vec<T>(t[h], static_cast<const T*>(g.d_y) + (int64_t)row * g.d_y_stride, c, p.columns);
+        load_weights<T>(w[h], p.weight, p.wide_weight, c, p.columns);
     };
     uint32_t turn = 0;
     inputs now, next;
@@ -255,28 +265,37 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
         if (AHEAD) {
             now = next;
             if (row + teams < p.rows) fetch(next, row + teams);
-        } else {
+        } else if (!LEAN) {
             fetch(now, row);
         }
         // one exchange for both: rstd comes from the sum of s^2, and mean(t n) = rstd mean(t s)
-        float squares = 0.0f, dot = 0.0f, n[HELD][VEC], t[HELD][VEC];
+        float squares = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
-            widen_vec<R>(n[h], now.s[h]);
-            widen_vec<T>(t[h], now.d_y[h]);
+            if (LEAN) {
+                again(h, row);
+            } else {
+                widen_vec<R>(n[h], now.s[h]);
+                widen_vec<T>(t[h], now.d_y[h]);
+            }
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 squares = fmaf(n[h][i], n[h][i], squares);
                 dot = fmaf(t[h][i] * w[h][i], n[h][i], dot);
             }
+            if (LEAN) __builtin_amdgcn_sched_barrier(0);
         }
         across<LANES, add_op>(squares, dot, lds[turn]);
         const float rstd = ovl_lane::rsq_(fmaf(squares, p.over_columns, p.eps));
         const float mean = dot * rstd * p.over_columns;
 #pragma unroll
         for (int h = 0; h < HELD; ++h) {
-            const uint32_t c = (h * LANES + lane) * VEC;
+            uint32_t c = (h * LANES + lane) * VEC;
             float out[VEC];
+            if (LEAN) {
+                again(h, row);
+                ovl_lane::keep(c);
+            }
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 const float unit = n[h][i] * rstd;
@@ -285,12 +304,14 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
             }
             if (g.d_summed != nullptr) {
                 float more[VEC];
-                widen_vec<R>(more, now.d_summed[h]);
+                if (LEAN) load_vec<R>(more, static_cast<const R*>(g.d_summed) + (int64_t)row * g.d_summed_stride, c, p.columns);
+                else widen_vec<R>(more, now.d_summed[h]);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) out[i] += more[i];
             }
             if (g.d_x != nullptr) store_vec<T>(out, static_cast<T*>(g.d_x) + row * p.columns, c, p.columns);
             if (g.d_residual != nullptr) store_vec<R>(out, static_cast<R*>(g.d_residual) + row * p.columns, c, p.columns);
+            if (LEAN) __builtin_amdgcn_sched_barrier(0);
         }
     }
 #pragma unroll

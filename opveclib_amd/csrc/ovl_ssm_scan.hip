@@ -759,8 +759,12 @@ template <int S> struct channel_sums {
 // as float32, one barrier per tile for them and one for the sums.
 //
 // Bound by the vector ALU: 26 instructions per token and 64 entries (14 of the recurrences, 4.5 of the sums over channels,
-// 2 of the states computed twice, the rest per token and channel), and the vector ALU is busy for 380 of the 490 us that
-// 4 sequences of 2048 tokens, 4096 channels of 16 entries in bf16 take.
+// 2 of the states computed twice, the rest per token and channel), and the vector ALU is busy for 380 of the 490 to 530 us
+// that 4 sequences of 2048 tokens, 4096 channels of 16 entries in bf16 take.
+//
+// SLICED: states of more than 16 entries are taken 16 at a time, tile by tile, and what a lane keeps of the other slices is
+// in LDS: with 8 or 16 entries in a lane only one wavefront fits a SIMD, or none without spilling (2048 channels of 32
+// entries 781 us and 620 in slices, of 64 entries 3289 and 1141; of 16 entries 320).
 template <typename T, int S, bool GATE, bool SLICED>
 __global__ void __launch_bounds__(THREADS) OVL_LANE_WAVES(2)
 scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, const float* entry) {
@@ -826,16 +830,6 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
         const uint32_t t0 = tile * TILE, left = p.length - t0, tokens = w.end - t0;
         T u_raw[QUADS], delta_raw[QUADS], z_raw[QUADS], dy_raw[QUADS], du_done[QUADS], ddelta_done[QUADS], dz_done[QUADS];
         float h_first[S];
-        auto fetch_slice = [&](uint32_t slice, stage& B_stage, stage& C_stage) {
-            if (left >= TILE) {
-                B_stage.load();
-                C_stage.load();
-            } else {
-                B_stage.load_some(left);
-                C_stage.load_some(left);
-            }
-            load_states(h_first, kept, (slice * 4u + w.q) * S, w.channel, p.channels);
-        };
         // Loaded here and not a tile ahead: the registers for that cost the second wavefront of a SIMD, which hides more
         // (261 registers and one wavefront: 690 us, 247 and two: 500 us for 4 x 2048 tokens of 4096 channels).
         if (left >= TILE) {
@@ -843,14 +837,22 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
             delta_from.load(delta_raw);
             dy_from.load(dy_raw);
             if (GATE) z_from.load(z_raw);
+            if (!SLICED) {
+                B_all.load();
+                C_all.load();
+            }
         } else {
             u_from.load_some(u_raw, left, w.q);
             delta_from.load_some(delta_raw, left, w.q);
             dy_from.load_some(dy_raw, left, w.q);
             if (GATE) z_from.load_some(z_raw, left, w.q);
+            if (!SLICED) {
+                B_all.load_some(left);
+                C_all.load_some(left);
+            }
         }
         if (!SLICED) {
-            fetch_slice(0u, B_all, C_all);
+            load_states(h_first, kept, w.q * S, w.channel, p.channels);
             B_all.store(lds_B, tokens, p.state);
             C_all.store(lds_C, tokens, p.state);
         }
@@ -901,7 +903,14 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
             const uint32_t first = slice * NP;
             if (SLICED) {
                 stage B_stage(p.B, w, threadIdx.x, t0, p.state, first), C_stage(p.C, w, threadIdx.x, t0, p.state, first);
-                fetch_slice(slice, B_stage, C_stage);
+                if (left >= TILE) {
+                    B_stage.load();
+                    C_stage.load();
+                } else {
+                    B_stage.load_some(left);
+                    C_stage.load_some(left);
+                }
+                load_states(h_first, kept, (slice * 4u + w.q) * S, w.channel, p.channels);
                 load_A2(slice);
                 B_stage.store(lds_B, tokens, p.state - first);
                 C_stage.store(lds_C, tokens, p.state - first);

@@ -69,7 +69,7 @@ static inline float rcp_(float x) { return 1.0f / x; }
 static inline float rsq_(float x) { return 1.0f / sqrtf(x); }
 
 static inline float positive(float x) { return x > 0.0f ? x : 0.0f; }
-static inline void keep(float&) {}
+template <typename X> static inline void keep(X&) {}
 static inline uint32_t anew(uint32_t x) { return x; }
 
 static inline uint32_t wavefront(uint32_t x) { return x; }
