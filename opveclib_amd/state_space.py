@@ -318,7 +318,8 @@ def _describe_scan(torch, u, delta, A, B, C, D, z, delta_bias, softplus, state, 
     scan_ = _pack_scan(batch, length, channels, n, groups, args.code, 1 if softplus else 0,
                        *args.sequence(u, 'u', shape), *args.sequence(delta, 'delta', shape), *args.sequence(z, 'z', shape),
                        *args.vectors(B, 'B', vector_shape, token, grouped),
-                       *args.vectors(C, 'C', vector_shape, token, grouped), args.parameter(A, 'A', (channels, n)), args.parameter(D, 'D', (channels,)),
+                       *args.vectors(C, 'C', vector_shape, token, grouped),
+                       args.parameter(A, 'A', (channels, n)), args.parameter(D, 'D', (channels,)),
                        args.parameter(delta_bias, 'delta_bias', (channels,)),
                        0 if token else args.parameter(state, 'state', (batch, channels, n)), args.lengths(lengths, batch))
     return args, scan_, (batch, length, channels, n)
