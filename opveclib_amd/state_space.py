@@ -425,6 +425,7 @@ def scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, softplu
         return y
     with args.on():
         _call(library().ovl_ssm_scan_step(scan_, state.data_ptr(), stride, y.data_ptr(), args.stream()))
+    torch.autograd.graph.increment_version(state)       # a backward pass that needs the state as it was raises
     return y
 
 
@@ -608,6 +609,7 @@ def conv_step(x, state, weight, bias=None, activation=None):
         return y
     with args.on():
         _call(library().ovl_ssm_conv_step(conv_, y.data_ptr(), args.stream()))
+    torch.autograd.graph.increment_version(state)       # a backward pass that needs the state as it was raises
     return y
 
 

@@ -356,6 +356,22 @@ def test_gradients_of_one_output_alone():
                 assert torch.equal(a, b)
 
 
+def test_a_state_that_a_backward_pass_needs_is_not_overwritten_unnoticed():
+    d = ref.scan_inputs(31, 2, 5, 12, 16, 1, 'float32', device='cuda')
+    c = ref.conv_inputs(31, 2, 5, 12, 4, 'float32', device='cuda')
+    u, x = d['u'].clone().requires_grad_(True), c['x'].clone().requires_grad_(True)
+    y, _ = state_space.scan_torch(u, d['delta'], d['A'], d['B'], d['C'], softplus=True, state=d['state'])
+    out, _ = state_space.conv_torch(x, c['weight'], c['bias'], 'silu', c['state'])
+    state_space.scan_step(d['state'], d['u'][:, 0], d['delta'][:, 0], d['A'], d['B'][:, 0], d['C'][:, 0], softplus=True)
+    state_space.conv_step(c['x'][:, 0], c['state'], c['weight'], c['bias'], 'silu')
+    for result in (y, out):
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            result.sum().backward()
+    with torch.inference_mode():
+        state = torch.zeros_like(d['state'])
+        state_space.scan_step(state, d['u'][:, 0], d['delta'][:, 0], d['A'], d['B'][:, 0], d['C'][:, 0], softplus=True)
+
+
 def test_sequences_without_tokens_and_batches_without_sequences():
     for batch, length in ((2, 0), (0, 5)):
         d = ref.scan_inputs(23, batch, length, 6, 4, 1, 'float32', device='cuda')
