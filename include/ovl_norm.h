@@ -6,7 +6,8 @@
  *   s[r,c] = x[r,c] + residual[r,c]   rounded to the residual's type, which is how it is stored; x[r,c] without a residual
  *   y[r,c] = s[r,c] * rstd[r] * weight[c]               rstd[r] = 1 / sqrt(mean over c of s[r,c]^2 + eps)
  *   q[r,c] = e4m3(y[r,c] / scale)                       scale = max |y| / 448 over the row, or over each 128 columns of it
- *                                                       (at least 2^-126, and 1 where all of them are zero)
+ *                                                       (at least 2^-126, and 1 where all of them are zero; NaN does not
+ *                                                       count), both of y in float32 before it is rounded to dtype
  *
  * The norm is that of the sum as stored, so that the layer that reads the sum later, and the backward pass, see the very
  * values that were normalised.  Sums and statistics are float32; y, q and s are rounded once.

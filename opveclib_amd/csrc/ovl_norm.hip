@@ -6,7 +6,8 @@
 //
 // Work layout: LANES lanes share a row (a wavefront, four or sixteen of them) and hold all of it in registers, HELD
 // vectors of eight columns per lane, so everything is read once and written once: the kernels are bound by memory.  The
-// statistics of a row are one exchange between its wavefronts.  Rows need not start on vector boundaries: the vectors are
+// statistics of a row are one exchange between its wavefronts, the largest result for a scale that spans the row another
+// (4096 rows of 20000 columns in bf16 with the residual: 155 us with the second, else 149).  Rows need not start on vector boundaries: the vectors are
 // accessed with the alignment of an element, a row's last, partial vector element by element.
 //
 // Measured: 16384 rows of 8192 columns in bf16 with the residual's addition, to 8 bits with a scale per 128 columns, 173 us
@@ -99,21 +100,36 @@ template <typename OP> __device__ __forceinline__ float wave_all(float x) {
     return OP::of(a, b);
 }
 
-// Two results over all lanes of a row of the matrix: a sum, and a second value by OP.  `lds` is not read again before
-// the next barrier after this call, so two calls need a barrier, or two places, between them.
+// Over all lanes of a row of the matrix; every lane receives the result.  `lds`, a number per wavefront, is not read again
+// before the next barrier after this call, so two calls need a barrier, or two places, between them.
 template <int LANES, typename OP>
-__device__ __forceinline__ void across(float& sum, float& other, float (*lds)[2]) {
-    sum = wave_all<add_op>(sum);
-    other = wave_all<OP>(other);
+__device__ __forceinline__ float across(float x, float* lds) {
+    x = wave_all<OP>(x);
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        if ((threadIdx.x & 63u) == 0u) lds[threadIdx.x / 64u] = x;
+        __syncthreads();
+        x = lds[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) x = OP::of(x, lds[i]);
+    }
+    return x;
+}
+
+// Two sums at a time, in the same way.
+template <int LANES>
+__device__ __forceinline__ void across(float& first, float& second, float (*lds)[2]) {
+    first = wave_all<add_op>(first);
+    second = wave_all<add_op>(second);
     if constexpr (LANES > 64) {
         constexpr int WAVES = LANES / 64;
         const uint32_t wave = threadIdx.x / 64u;
-        if ((threadIdx.x & 63u) == 0u) { lds[wave][0] = sum; lds[wave][1] = other; }
+        if ((threadIdx.x & 63u) == 0u) { lds[wave][0] = first; lds[wave][1] = second; }
         __syncthreads();
-        sum = lds[0][0];
-        other = lds[0][1];
+        first = lds[0][0];
+        second = lds[0][1];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) { sum += lds[i][0]; other = OP::of(other, lds[i][1]); }
+        for (int i = 1; i < WAVES; ++i) { first += lds[i][0]; second += lds[i][1]; }
     }
 }
 
@@ -131,7 +147,7 @@ template <typename T, typename R, int LANES, int HELD, bool QUANTIZED, bool GROU
 __global__ void __launch_bounds__(LANES > 256 ? LANES : 256)
 norm_forward_kernel(norm_args p, T* y, R* summed, uint8_t* q, float* scales) {
     constexpr uint32_t PER = LANES > 256 ? 1 : 256 / LANES;     // rows of a workgroup
-    __shared__ float lds[LANES / 64][2];
+    __shared__ float lds[2][LANES / 64];
     const uint32_t lane = threadIdx.x % LANES;
     const uint64_t row = (uint64_t)blockIdx.x * PER + threadIdx.x / LANES;
     if (row >= p.rows) return;              // with more than one row per workgroup there is no barrier
@@ -152,58 +168,71 @@ norm_forward_kernel(norm_args p, T* y, R* summed, uint8_t* q, float* scales) {
             store_vec<R>(s[h], to, c, p.columns);
         }
     }
-    float squares = 0.0f, largest = 0.0f;
+    float squares = 0.0f;
 #pragma unroll
     for (int h = 0; h < HELD; ++h)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) squares = fmaf(s[h][i], s[h][i], squares);
     float w[HELD][VEC];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
-        if (QUANTIZED && !GROUPED)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) largest = fmaxf(largest, fabsf(s[h][i] * w[h][i]));
-    }
-    across<LANES, max_op>(squares, largest, lds);
+    for (int h = 0; h < HELD; ++h) load_weights<T>(w[h], p.weight, p.wide_weight, (h * LANES + lane) * VEC, p.columns);
+    squares = across<LANES, add_op>(squares, lds[0]);
     const float rstd = ovl_lane::rsq_(fmaf(squares, p.over_columns, p.eps));
-    // one scale for the row: max |y| = rstd max |s w|
-    // (a scale below the smallest normal number is taken as that: its reciprocal would not be finite)
-    auto scale_of = [](float top) { return top > 0.0f ? fmaxf(top / E4M3_MAX, 0x1p-126f) : 1.0f; };
-    const float row_largest = largest * rstd;
-    if (QUANTIZED && !GROUPED && lane == 0u) scales[row] = scale_of(row_largest);
+    if constexpr (!QUANTIZED) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            float out[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) out[i] = s[h][i] * rstd * w[h][i];
+            store_vec<T>(out, y + row * p.columns, (h * LANES + lane) * VEC, p.columns);
+        }
+        return;
+    }
+    float row_top = 0.0f;                   // s becomes y
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            s[h][i] = s[h][i] * rstd * w[h][i];
+            if (!GROUPED) row_top = fmaxf(row_top, fabsf(s[h][i]));
+        }
+    // The smallest scale is the smallest normal number: the last bits of one below would not be there.  y is divided by it: a
+    // product with a rounded reciprocal would move values in the middle of two e4m3 numbers, so the reciprocal is carried to
+    // twice the precision, which makes the product the rounded quotient (where the low part is a normal number, for scales
+    // up to 2^100).
+    float scale, high, low;
+    auto scale_by = [&](float top) {
+        scale = top > 0.0f ? fmaxf(top / E4M3_MAX, 0x1p-126f) : 1.0f;
+        high = ovl_lane::rcp_(scale);
+        low = scale <= 0x1p100f ? fmaf(-high, scale, 1.0f) * high : 0.0f;
+    };
+    if (!GROUPED) {
+        scale_by(across<LANES, max_op>(row_top, lds[1]));
+        if (lane == 0u) scales[row] = scale;
+    }
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
         const uint32_t c = (h * LANES + lane) * VEC;
+        if (GROUPED) {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(s[h][i]));
+            scale_by(row_all<max_op>(top));
+            const uint32_t group = c / 128u, groups = (p.columns + 127u) / 128u;
+            if ((lane & 15u) == 0u && group < groups) scales[row * groups + group] = scale;
+        }
         float out[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) out[i] = s[h][i] * rstd * w[h][i];
-        if constexpr (!QUANTIZED) {
-            store_vec<T>(out, y + row * p.columns, c, p.columns);
-        } else {
-            float top = row_largest;
-            if constexpr (GROUPED) {
-                top = 0.0f;
+        for (int i = 0; i < VEC; ++i) out[i] = fmaf(s[h][i], high, s[h][i] * low);
+        struct __attribute__((packed, aligned(1))) bytes { uint32_t v[2]; } packed;
+        packed.v[0] = ovl_lane::e4m3x4(out[0], out[1], out[2], out[3]);
+        packed.v[1] = ovl_lane::e4m3x4(out[4], out[5], out[6], out[7]);
+        uint8_t* to = q + row * p.columns + c;
+        if (c + VEC <= p.columns) *reinterpret_cast<bytes*>(to) = packed;
+        else
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(out[i]));
-                top = row_all<max_op>(top);
-                const uint32_t group = c / 128u, groups = (p.columns + 127u) / 128u;
-                if ((lane & 15u) == 0u && group < groups)
-                    scales[row * groups + group] = scale_of(top);
-            }
-            const float inverse = top > 0.0f ? fminf(E4M3_MAX / top, 0x1p126f) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) out[i] *= inverse;
-            struct __attribute__((packed, aligned(1))) bytes { uint32_t v[2]; } packed;
-            packed.v[0] = ovl_lane::e4m3x4(out[0], out[1], out[2], out[3]);
-            packed.v[1] = ovl_lane::e4m3x4(out[4], out[5], out[6], out[7]);
-            uint8_t* to = q + row * p.columns + c;
-            if (c + VEC <= p.columns) *reinterpret_cast<bytes*>(to) = packed;
-            else
-#pragma unroll
-                for (uint32_t i = 0; i < VEC; ++i)
-                    if (c + i < p.columns) to[i] = (uint8_t)(packed.v[i / 4u] >> (8u * (i % 4u)));
-        }
+            for (uint32_t i = 0; i < VEC; ++i)
+                if (c + i < p.columns) to[i] = (uint8_t)(packed.v[i / 4u] >> (8u * (i % 4u)));
     }
 }
 
@@ -285,7 +314,7 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
             }
             if (LEAN) __builtin_amdgcn_sched_barrier(0);
         }
-        across<LANES, add_op>(squares, dot, lds[turn]);
+        across<LANES>(squares, dot, lds[turn]);
         const float rstd = ovl_lane::rsq_(fmaf(squares, p.over_columns, p.eps));
         const float mean = dot * rstd * p.over_columns;
 #pragma unroll

@@ -196,9 +196,10 @@ def rms_norm(x, weight, eps=1e-5, residual=None):
 
 def rms_norm_quantized(x, weight, eps=1e-5, residual=None, group=None):
     """
-    :func:`rms_norm` with its result in 8 bits: ``q = e4m3(y / scale)``, rounded once from float32, where scale is the
-    largest magnitude of y divided by 448 (the largest e4m3 value) - of the row, or with ``group=128`` of each 128 columns
-    of it -, at least 2^-126 (the smallest normal number), and 1 where all of them are zero.
+    :func:`rms_norm` with its result in 8 bits: ``q = e4m3(y / scale)``, the float32 quotient of the float32 result y
+    rounded to nearest, ties to even, where scale is the largest magnitude of y divided by 448 (the largest e4m3 value) - of
+    the row, or with ``group=128`` of each 128 columns of it -, at least 2^-126 (the smallest normal number), and 1 where all
+    of them are zero (NaN does not count).
 
     :return: (q, scales) with q a torch.float8_e4m3fn tensor like ``x`` and scales [..., 1] resp. [..., ceil(columns /
         128)] in float32; with a residual (q, scales, s)

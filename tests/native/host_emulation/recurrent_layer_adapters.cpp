@@ -82,7 +82,7 @@ extern "C" int emu_recurrent_layer(const ovl_tensor* in, uint32_t n_in, ovl_tens
     } else if (s[0] >= 6 && s[0] <= 8) {
         ovl_norm p = {};
         p.rows = (uint32_t)s[1]; p.columns = (uint32_t)s[2]; p.dtype = (int32_t)s[3]; p.residual_dtype = (int32_t)s[4];
-        p.weight_dtype = (int32_t)s[5]; p.eps = 1e-5f;
+        p.weight_dtype = (int32_t)s[5]; p.eps = s[0] == 7 && in[0].len > 9 ? 0.0f : 1e-5f;
         p.x = at(in[1]); p.x_stride = s[6];
         p.residual = at(in[2]); p.residual_stride = s[7];
         p.weight = at(in[3]);

@@ -109,6 +109,28 @@ def scales_of(y, group=None):
     return torch.where(scale > 0, scale, torch.ones_like(scale))
 
 
+def quantized(y, group=None):
+    """The codes and scales that float32 results of the norm have to get, bit for bit: the largest magnitude divided by 448,
+    at least 2^-126, and the quotients rounded to e4m3 (division and rounding of the CPU)."""
+    y = y.detach().cpu()
+    parts = y.split(group or y.shape[-1], -1)
+    scales = torch.stack([p.abs().amax(-1) / E4M3_MAX for p in parts], -1).clamp(min=2.0 ** -126)
+    scales = torch.where(torch.stack([p.abs().amax(-1) for p in parts], -1) > 0, scales, torch.ones_like(scales))
+    each = scales.repeat_interleave(group or y.shape[-1], -1)[..., :y.shape[-1]]
+    return (y / each).to(torch.float8_e4m3fn), scales
+
+
+def middles(divisors):
+    """For each of the divisors d (odd whole numbers of up to 19 bits) a row of 128 float32 weights whose results, for rows of
+    ones without eps, are the weights themselves: 448 d, which makes the scale d, and then t d for numbers t in the middle of
+    two neighbouring e4m3 numbers.  Both products are exact, so every quotient is such a middle and goes to the even one."""
+    t = torch.tensor([(2 * m + 1) * 2.0 ** e for e in range(-4, 5) for m in range(8, 16)], dtype=torch.float64)
+    t = torch.cat([torch.tensor([448.0], dtype=torch.float64), t[t < 448], torch.ones(128, dtype=torch.float64)])[:128]
+    rows = torch.tensor(divisors, dtype=torch.float64)[:, None] * t
+    assert torch.equal(rows.float().double(), rows)
+    return rows.float(), t
+
+
 def scan_inputs(seed, batch, length, channels, n, groups, dtype, gate=True, ragged=False, entering=True, device='cpu',
                 softplus=True, skip=True, bias=True):
     """Inputs of the sizes a layer meets; softplus leaves time steps between 0.001 and 0.3."""

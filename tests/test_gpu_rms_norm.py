@@ -223,3 +223,27 @@ def test_matrices_beyond_32_bits_of_bytes():
     assert torch.equal(q[-64:].view(torch.uint8), tail.view(torch.uint8)) and torch.equal(scales[-64:], tail_scales)
     d_x, _, _ = rms_norm.rms_norm_grad(x, w, y)
     assert torch.equal(d_x[-64:], rms_norm.rms_norm_grad(x[-64:].contiguous(), w, y[-64:].contiguous())[0])
+
+
+@pytest.mark.parametrize('rows,columns', [(3000, 100), (700, 1000), (300, 4096), (40, 20001)])
+def test_codes_and_scales_are_those_of_the_results(rows, columns):
+    """Bit for bit: the results of rms_norm in float32 divided on the CPU, for both kinds of scales."""
+    x, _, _, _, _ = inputs(7, (rows, columns), 'float32', None, 'float32')
+    w = torch.randn(columns, device='cuda')
+    y = rms_norm.rms_norm(x, w)
+    for group in (None, 128):
+        q, scales = rms_norm.rms_norm_quantized(x, w, group=group)
+        want, want_scales = ref.quantized(y, group)
+        assert torch.equal(scales.cpu(), want_scales)
+        assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8))
+
+
+def test_middles_of_two_8_bit_numbers_go_to_the_even_one():
+    weights, t = ref.middles(list(range(1, 200, 2)) + [1021, 65537, 262657])
+    want = t.float().to(torch.float8_e4m3fn).view(torch.uint8).cuda()
+    ones = torch.ones(2, 128, device='cuda')
+    for row in weights:
+        for group in (None, 128):
+            q, scales = rms_norm.rms_norm_quantized(ones, row.cuda(), eps=0.0, group=group)
+            assert bool((scales == row[0].item() / 448).all())
+            assert torch.equal(q.view(torch.uint8), want.expand(2, 128))

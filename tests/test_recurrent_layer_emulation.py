@@ -260,3 +260,33 @@ def test_norm(program, case):
     close(d_x, want[0], kind, 'd_x', 16)
     close(d_r, want[0], r_kind, 'd_residual', 16)
     close(d_w, want[1], weight.dtype, 'd_weight', 16)
+
+
+@pytest.mark.parametrize('rows,columns', [(12, 120), (2, 515), (1, 2052)])
+def test_norm_to_8_bits_divides_its_own_results(program, rows, columns):
+    """Codes and scales are those of the float32 results, bit for bit, and rows of up to 128 columns get the same from both
+    forms."""
+    g = torch.Generator()
+    g.manual_seed(7)
+    x = torch.randn(rows, columns, generator=g)
+    weight = torch.randn(columns, generator=g)
+    settings = [rows, columns, 2, 2, 2, columns, columns]
+    none = ((0,), torch.float32)
+    y, _ = run(program, [6] + settings, [x, None, weight], [((rows, columns), torch.float32), none])
+    for group in (0, 128):
+        q, scales, _ = run(program, [7] + settings + [group], [x, None, weight],
+                           [((rows, columns), torch.float8_e4m3fn), ((rows, -(-columns // 128) if group else 1), torch.float32), none])
+        want, want_scales = ref.quantized(y, group or None)
+        assert torch.equal(scales, want_scales)
+        assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
+
+
+def test_norm_to_8_bits_sends_middles_to_the_even_number(program):
+    weights, t = ref.middles([1, 3, 5, 7, 11, 49, 1021, 65537, 262657])
+    ones = torch.ones(1, 128)
+    for row in weights:
+        for group in (0, 128):
+            q, scales, _ = run(program, [7, 1, 128, 2, 2, 2, 128, 128, group, 1], [ones, None, row],
+                               [((1, 128), torch.float8_e4m3fn), ((1, 1), torch.float32), ((0,), torch.float32)])
+            assert scales.item() == row[0].item() / 448
+            assert torch.equal(q.view(torch.uint8)[0], t.float().to(torch.float8_e4m3fn).view(torch.uint8))
