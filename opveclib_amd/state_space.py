@@ -454,9 +454,10 @@ def _differentiable(name):
 
     class _Scan(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, u, delta, A, B, C, D, z, delta_bias, state, lengths, softplus):
+        def forward(ctx, u, delta, A, B, C, D, z, delta_bias, state, lengths, softplus, recorded):
+            # (needs_input_grad follows the tensors alone, also where nothing is recorded)
             y, last, saved = _scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths,
-                                   any(ctx.needs_input_grad))
+                                   recorded and any(ctx.needs_input_grad))
             ctx.softplus = softplus
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, state, lengths, saved)
@@ -469,7 +470,7 @@ def _differentiable(name):
             if d_y is None:
                 d_y = torch.zeros_like(u)
             grads = scan_grad(u, delta, A, B, C, d_y, D, z, delta_bias, ctx.softplus, state, lengths, d_last, saved)
-            return grads + (None, None)
+            return grads + (None, None, None)
 
     class _Conv(torch.autograd.Function):
         @staticmethod
@@ -493,9 +494,12 @@ def _differentiable(name):
 
 
 def scan_torch(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False, state=None, lengths=None):
-    """:func:`scan` as a differentiable PyTorch function.  Where a gradient is wanted the forward pass keeps the state
-    before every 16th token (4 * state / 16 bytes for each element of ``u``) for the backward pass."""
-    return _differentiable('scan').apply(u, delta, A, B, C, D, z, delta_bias, state, lengths, softplus)
+    """:func:`scan` as a differentiable PyTorch function.  Where a backward pass can follow (an input requires a gradient,
+    outside of ``torch.no_grad()`` and the like) the forward pass keeps the state before every 16th token for it: for each
+    element of ``u`` 4 / 16 bytes times the state entries, counted as the next of 8, 16, 32 or 64."""
+    import torch
+    return _differentiable('scan').apply(u, delta, A, B, C, D, z, delta_bias, state, lengths, softplus,
+                                         torch.is_grad_enabled())
 
 
 # ----------------------------------------------------------------------------------------------------------------------

@@ -196,3 +196,25 @@ def test_calls_pack_their_structs_as_the_headers_lay_them_out():
     same(state_space._pack_sequence(*v), state_space.Sequence(*v))
     v = some(5) + [0.25] + some(5)
     same(rms_norm._pack(*v), rms_norm.Norm(*v))
+
+
+def test_scan_torch_keeps_states_only_where_a_backward_pass_can_follow(monkeypatch):
+    kept = []
+
+    def scan_without_a_gpu(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, keep):
+        kept.append(keep)
+        return u * 1, u.new_zeros(u.shape[0], u.shape[2], A.shape[1]), u.new_zeros(1) if keep else None
+
+    monkeypatch.setattr(state_space, '_scan', scan_without_a_gpu)
+    u, B, plain = torch.zeros(2, 4, 8), torch.zeros(2, 4, 3), torch.zeros(8, 3)
+    A = torch.nn.Parameter(torch.zeros(8, 3))
+    y, _ = state_space.scan_torch(u, u, A, B, B)
+    assert kept.pop() and y.requires_grad
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            y, _ = state_space.scan_torch(u, u, A, B, B)
+        assert not kept.pop() and not y.requires_grad
+    y, _ = state_space.scan_torch(u, u, plain, B, B)
+    assert not kept.pop() and not y.requires_grad
+    y, _ = state_space.scan_torch(u, u, plain, B, B, state=torch.zeros(2, 8, 3, requires_grad=True))
+    assert kept.pop() and y.requires_grad
