@@ -238,6 +238,16 @@ def test_codes_and_scales_are_those_of_the_results(rows, columns):
         assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8))
 
 
+def test_zeros_keep_their_sign_in_8_bits():
+    x = torch.randn(500, 64, device='cuda')
+    x[:, ::3] = 0
+    x = torch.where(torch.rand_like(x) < 0.5, -x, x)
+    w = 0.1 + torch.rand(64, device='cuda')
+    for group in (None, 128):
+        q, _ = rms_norm.rms_norm_quantized(x, w, group=group)
+        assert torch.equal(q.view(torch.uint8) >= 128, torch.signbit(x))
+
+
 def test_middles_of_two_8_bit_numbers_go_to_the_even_one():
     weights, t = ref.middles(list(range(1, 200, 2)) + [1021, 65537, 262657])
     want = t.float().to(torch.float8_e4m3fn).view(torch.uint8).cuda()

@@ -281,6 +281,15 @@ def test_norm_to_8_bits_divides_its_own_results(program, rows, columns):
         assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
 
 
+def test_norm_to_8_bits_keeps_the_sign_of_zeros(program):
+    x = torch.tensor([[0.0, -0.0, 3.0, -2.0] * 4, [-0.0, 0.0, -1.7, 2.0] * 4])
+    for top in (3.0, 1.9, 1.1, 0.7):
+        for group in (0, 128):
+            q, _, _ = run(program, [7, 2, 16, 2, 2, 2, 16, 16, group], [x, None, torch.full((16,), top)],
+                          [((2, 16), torch.float8_e4m3fn), ((2, 1), torch.float32), ((0,), torch.float32)])
+            assert torch.equal(q.view(torch.uint8) >= 128, torch.signbit(x))
+
+
 def test_norm_to_8_bits_sends_middles_to_the_even_number(program):
     weights, t = ref.middles([1, 3, 5, 7, 11, 49, 1021, 65537, 262657])
     ones = torch.ones(1, 128)
