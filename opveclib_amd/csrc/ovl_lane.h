@@ -15,6 +15,9 @@
 
 namespace ovl_lane {
 
+// Work items of one launch: HIP takes fewer than 2^32.
+constexpr uint64_t MOST_WORK_ITEMS = 0xffffffff;
+
 typedef _Float16 f16;
 typedef __bf16 bf16;
 

@@ -397,7 +397,6 @@ int check(const char* who, const ovl_norm* p) {
     if (p == nullptr) return fail(name + ": null norm");
     if (p->rows == 0 || p->columns == 0) return fail(name + ": sizes must be positive");
     if (p->columns > 32768u) return fail(name + ": at most 32768 columns");
-    if (p->rows > (1u << 31) - 1u) return fail(name + ": too many rows for one launch");
     if (!known(p->dtype)) return fail(name + ": unknown element type");
     if (p->residual_dtype != p->dtype && p->residual_dtype != OVL_NORM_FLOAT32) return fail(name + ": the residual must be of the rows' type or float32");
     if (p->weight_dtype != p->dtype && p->weight_dtype != OVL_NORM_FLOAT32) return fail(name + ": the weight must be of the rows' type or float32");
@@ -436,6 +435,26 @@ template <typename F> void by_types(const ovl_norm* p, F&& call) {
     }
 }
 
+// Calls launch(first row, rows, workgroups) for pieces of the matrix that one launch can take: a row of up to 2048 columns
+// is 64 work items, so 2^26 rows are too many.
+template <typename F> void by_pieces(uint32_t rows, uint32_t threads, uint32_t per_workgroup, F&& launch) {
+    const uint64_t most = ovl_lane::MOST_WORK_ITEMS / threads * per_workgroup;
+    for (uint64_t first = 0; first < rows; first += most) {
+        const uint32_t here = (uint32_t)(rows - first < most ? rows - first : most);
+        launch(first, here, (here + per_workgroup - 1) / per_workgroup);
+    }
+}
+
+// The arguments of the rows from `first` on.
+norm_args piece_of(const ovl_norm* p, uint64_t first, uint32_t rows) {
+    norm_args args = make_args(p);
+    args.rows = rows;
+    const int64_t size = p->dtype == OVL_NORM_FLOAT32 ? 4 : 2, residual_size = p->residual_dtype == OVL_NORM_FLOAT32 ? 4 : 2;
+    args.x = static_cast<const char*>(p->x) + (int64_t)first * p->x_stride * size;
+    if (p->residual != nullptr) args.residual = static_cast<const char*>(p->residual) + (int64_t)first * p->residual_stride * residual_size;
+    return args;
+}
+
 template <int LANES> constexpr uint32_t threads_of() { return LANES > 256 ? LANES : 256; }
 
 // Teams of the backward pass: two workgroups per compute unit (of 1024 lanes one); a team's part of the weight gradient
@@ -443,7 +462,7 @@ template <int LANES> constexpr uint32_t threads_of() { return LANES > 256 ? LANE
 // with float32 sums), 125 for 112 at 32768 of 1000, but 63 for 71 at 65536 of 512 all in bf16.
 uint32_t teams_for(const ovl_norm* p) {
     const uint32_t most = p->columns <= 2048u ? 2048u : p->columns <= 8192u ? 512u : 256u;
-    const uint32_t few = (p->rows + 3u) / 4u;
+    const uint32_t few = (uint32_t)((p->rows + 3ull) / 4u);
     return few < most ? few : most;
 }
 
@@ -458,16 +477,19 @@ int ovl_norm_forward(const ovl_norm* p, void* y, void* summed, void* hip_stream)
     if (rc != OVL_OK) return rc;
     if (y == nullptr || (p->residual != nullptr && summed == nullptr)) return fail("ovl_norm_forward: null tensor");
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
-    const norm_args args = make_args(p);
     by_types(p, [&](auto t, auto r) {
         typedef decltype(t) T;
         typedef decltype(r) R;
         by_columns(p->columns, [&](auto lanes, auto held) {
             constexpr int LANES = decltype(lanes)::value, HELD = decltype(held)::value;
             constexpr uint32_t THREADS = threads_of<LANES>(), PER = THREADS / LANES;
-            hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, false, false>), dim3((p->rows + PER - 1) / PER),
-                               dim3(THREADS), 0, stream, args, static_cast<T*>(y), static_cast<R*>(summed),
-                               static_cast<uint8_t*>(nullptr), static_cast<float*>(nullptr));
+            by_pieces(p->rows, THREADS, PER, [&](uint64_t first, uint32_t rows, uint32_t workgroups) {
+                const norm_args args = piece_of(p, first, rows);
+                T* to = static_cast<T*>(y) + first * p->columns;
+                R* sum = summed != nullptr ? static_cast<R*>(summed) + first * p->columns : nullptr;
+                hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, false, false>), dim3(workgroups), dim3(THREADS), 0,
+                                   stream, args, to, sum, static_cast<uint8_t*>(nullptr), static_cast<float*>(nullptr));
+            });
         });
     });
     return after_launch("ovl_norm_forward");
@@ -482,22 +504,26 @@ int ovl_norm_forward_quantized(const ovl_norm* p, uint32_t group_columns, void* 
     if (q == nullptr || scales == nullptr || (p->residual != nullptr && summed == nullptr))
         return fail("ovl_norm_forward_quantized: null tensor");
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
-    const norm_args args = make_args(p);
+    const uint64_t groups = group_columns != 0u ? (p->columns + 127u) / 128u : 1u;
     by_types(p, [&](auto t, auto r) {
         typedef decltype(t) T;
         typedef decltype(r) R;
         by_columns(p->columns, [&](auto lanes, auto held) {
             constexpr int LANES = decltype(lanes)::value, HELD = decltype(held)::value;
             constexpr uint32_t THREADS = threads_of<LANES>(), PER = THREADS / LANES;
-            const dim3 grid((p->rows + PER - 1) / PER);
-            if (group_columns != 0u)
-                hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, true, true>), grid, dim3(THREADS), 0, stream, args,
-                                   static_cast<T*>(nullptr), static_cast<R*>(summed),
-                                   static_cast<uint8_t*>(q), scales);
-            else
-                hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, true, false>), grid, dim3(THREADS), 0, stream, args,
-                                   static_cast<T*>(nullptr), static_cast<R*>(summed),
-                                   static_cast<uint8_t*>(q), scales);
+            by_pieces(p->rows, THREADS, PER, [&](uint64_t first, uint32_t rows, uint32_t workgroups) {
+                const norm_args args = piece_of(p, first, rows);
+                R* sum = summed != nullptr ? static_cast<R*>(summed) + first * p->columns : nullptr;
+                uint8_t* to = static_cast<uint8_t*>(q) + first * p->columns;
+                float* to_scales = scales + first * groups;
+                const dim3 grid(workgroups);
+                if (group_columns != 0u)
+                    hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, true, true>), grid, dim3(THREADS), 0, stream, args,
+                                       static_cast<T*>(nullptr), sum, to, to_scales);
+                else
+                    hipLaunchKernelGGL((norm_forward_kernel<T, R, LANES, HELD, true, false>), grid, dim3(THREADS), 0, stream, args,
+                                       static_cast<T*>(nullptr), sum, to, to_scales);
+            });
         });
     });
     return after_launch("ovl_norm_forward_quantized");

@@ -13,6 +13,9 @@ static inline uint32_t max(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
 namespace ovl_lane {
 
+// few, so that calls that take several launches are tried
+constexpr uint64_t MOST_WORK_ITEMS = 2048;
+
 struct bf16 { uint16_t bits; };
 struct f16 { uint16_t bits; };
 

@@ -257,3 +257,24 @@ def test_middles_of_two_8_bit_numbers_go_to_the_even_one():
             q, scales = rms_norm.rms_norm_quantized(ones, row.cuda(), eps=0.0, group=group)
             assert bool((scales == row[0].item() / 448).all())
             assert torch.equal(q.view(torch.uint8), want.expand(2, 128))
+
+
+def test_more_rows_than_one_launch_takes():
+    """2^26 rows of 64 work items."""
+    rows, columns = 2 ** 26 + 5, 8
+    x = torch.randn(1024, columns, device='cuda').bfloat16().repeat(rows // 1024 + 1, 1)[:rows]
+    r = torch.randn(rows, columns, device='cuda').bfloat16()
+    w = torch.randn(columns, device='cuda')
+    y, s = rms_norm.rms_norm(x, w, residual=r)
+    d_x, _, d_w = rms_norm.rms_norm_grad(s, w, x)
+    for part in (slice(0, 300), slice(2 ** 26 - 8, 2 ** 26 + 5), slice(12345678, 12345700)):
+        want_y, want_s = rms_norm.rms_norm(x[part].clone(), w, residual=r[part].clone())
+        assert torch.equal(y[part], want_y) and torch.equal(s[part], want_s)
+        assert torch.equal(d_x[part], rms_norm.rms_norm_grad(s[part].clone(), w, x[part].clone())[0])
+    assert torch.equal(s, x + r)
+    assert torch.isfinite(y).all() and torch.isfinite(d_w).all()
+    for group in (None, 128):
+        q, scales = rms_norm.rms_norm_quantized(s, w, group=group)
+        want, want_scales = ref.quantized(rms_norm.rms_norm(s[-4000:].float(), w), group)
+        assert torch.equal(scales[-4000:].cpu(), want_scales)
+        assert torch.equal(q[-4000:].cpu().view(torch.uint8), want.view(torch.uint8))

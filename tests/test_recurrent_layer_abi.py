@@ -218,3 +218,11 @@ def test_scan_torch_keeps_states_only_where_a_backward_pass_can_follow(monkeypat
     assert not kept.pop() and not y.requires_grad
     y, _ = state_space.scan_torch(u, u, plain, B, B, state=torch.zeros(2, 8, 3, requires_grad=True))
     assert kept.pop() and y.requires_grad
+
+
+def test_norms_of_any_number_of_rows_are_taken(libraries):
+    """Forward passes of many rows are several launches; the backward pass walks."""
+    _, lib = libraries
+    for rows in ((1 << 26) + 1, (1 << 31) + 1, (1 << 32) - 1):
+        s = rms_norm.Norm(rows, 64, 32, 32, 2, 1e-5, P, 64, None, 0, P)
+        assert lib.ovl_norm_workspace_bytes(ctypes.byref(s)) == 2048 * 64 * 4, rows

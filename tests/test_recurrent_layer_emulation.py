@@ -299,3 +299,29 @@ def test_norm_to_8_bits_sends_middles_to_the_even_number(program):
                                [((1, 128), torch.float8_e4m3fn), ((1, 1), torch.float32), ((0,), torch.float32)])
             assert scales.item() == row[0].item() / 448
             assert torch.equal(q.view(torch.uint8)[0], t.float().to(torch.float8_e4m3fn).view(torch.uint8))
+
+
+@pytest.mark.parametrize('rows,columns', [(70, 24), (9, 2060), (5, 9001)])
+def test_norm_in_several_launches(program, rows, columns):
+    """The emulated device takes 2048 work items in a launch: 32, 8 and 2 rows of these."""
+    g = torch.Generator()
+    g.manual_seed(8)
+    x, r = torch.randn(rows, columns, generator=g).bfloat16(), torch.randn(rows, columns + 3, generator=g)
+    weight = torch.randn(columns, generator=g).bfloat16()
+    b16, f32 = torch.bfloat16, torch.float32
+    s = x.float() + r[:, :columns]
+    want = ref.norm(s.double(), weight.double())
+    settings = [rows, columns, ref.CODES['bfloat16'], ref.CODES['float32'], ref.CODES['bfloat16'], columns, columns + 3]
+    y, summed = run(program, [6] + settings, [x, r, weight], [((rows, columns), b16), ((rows, columns), f32)])
+    close(y, want, b16, 'y', 4)
+    assert torch.equal(summed, s)
+    for group in (0, 128):
+        scale_shape = (rows, -(-columns // 128) if group else 1)
+        q, scales, summed = run(program, [7] + settings + [group], [x, r, weight],
+                                [((rows, columns), torch.float8_e4m3fn), (scale_shape, f32), ((rows, columns), f32)])
+        assert torch.equal(summed, s)
+        want_scales = ref.scales_of(want, group or None)
+        close(scales, want_scales, f32, 'scales', 4)
+        exact = want / want_scales.repeat_interleave(group or columns, 1)[:, :columns]
+        # one rounding to four significant bits (2^-10 in the subnormal range), and float32 arithmetic before it
+        assert bool(((q.double() - exact).abs() <= exact.abs() * (2.0 ** -4 + 2.0 ** -20) + 2.0 ** -10).all())
