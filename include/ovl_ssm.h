@@ -23,8 +23,17 @@
  * side, batch and token strides (in elements) are free, but for the scan's token strides, which are 0 to 2^25; outputs are
  * dense.  All sums, states and gradients of parameters are float32; only what is stored in the tensors' type is rounded,
  * once.  The functions enqueue kernels on `hip_stream`, return without synchronising, allocate nothing (scratch memory is
- * handed in, its size is asked for first) and give the same bits for the same call.  They return an ovl_status (ovl_launch.h): OVL_EINVAL for arguments
- * they refuse, OVL_EHIP for a HIP error (text from ovl_ssm_last_error).
+ * handed in, its size is asked for first) and give the same bits for the same call.  They return an ovl_status
+ * (ovl_launch.h): OVL_EINVAL for arguments they refuse, OVL_EHIP for a HIP error (text from ovl_ssm_last_error).
+ *
+ * Sizes: lengths up to 2^30, scans up to 2^22 channels, and what one launch takes (fewer than 2^32 work items), which is
+ *   scan           batch * groups * ceil(channels / groups / 64) below 2^26; backward pass and step (there without groups)
+ *                  below 2^24
+ *                  backward pass also 2 * groups * batch * length * state + 1024 * ceil(channels * (entries + 2) / 64) below
+ *                  2^32, entries = the state counted as the next of 8, 16, 32, 64
+ *   convolution    batch * channels below 2^32, up to 8 times as much where wide accesses are possible; backward pass
+ *                  channels * (width + 1) below 2^28, and batch * channels below 2^29 (more where channels are many)
+ * Larger calls are refused.
  */
 #ifndef OVL_SSM_H_
 #define OVL_SSM_H_

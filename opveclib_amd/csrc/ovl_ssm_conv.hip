@@ -365,7 +365,7 @@ conv_step_kernel(conv_args<T> p, uint32_t vectors, T* kept, T* y) {
 
 using ovl_ssm::after_launch;
 using ovl_ssm::fail;
-using ovl_ssm::round_up;
+using ovl_ssm::launchable;
 
 uint32_t size_of(int32_t dtype) { return dtype == OVL_SSM_FLOAT32 ? 4u : 2u; }
 
@@ -384,6 +384,12 @@ int check(const char* who, const ovl_ssm_conv* s, bool token) {
     if ((uint64_t)s->batch * s->length > ((1ull << 31) - 1) * THREADS / s->channels)
         return fail(OVL_SSM_EINVAL, name + ": too many elements for one launch");
     return OVL_SSM_OK;
+}
+
+// Whether a lane for `vec` channels of every sequence can be launched (the forward pass has more only where that is few).
+int check_lanes(const char* who, const ovl_ssm_conv* s, uint32_t vec) {
+    if (launchable(((uint64_t)s->batch * (s->channels / vec) + THREADS - 1) / THREADS, THREADS)) return OVL_SSM_OK;
+    return fail(OVL_SSM_EINVAL, std::string(who) + ": too many elements for one launch");
 }
 
 // The widest access (in elements, at most 16 bytes) that the channel count, the strides and the addresses allow.
@@ -449,6 +455,9 @@ cut cut_for(const ovl_ssm_conv* s, uint32_t vec) {
     return k;
 }
 
+// Workgroups of conv_sum_kernel for a tap.
+uint32_t sum_columns(const ovl_ssm_conv* s) { return s->channels / 64u + (s->channels % 64u != 0u); }
+
 template <typename T, int W, int VEC>
 void backward(const ovl_ssm_conv* s, const ovl_ssm_sequence* d_y, const ovl_ssm_sequence* d_last, T* d_x, T* d_kept,
               float* d_weight, float* d_bias, float* part, hipStream_t stream) {
@@ -462,7 +471,7 @@ void backward(const ovl_ssm_conv* s, const ovl_ssm_sequence* d_y, const ovl_ssm_
     g.part = part;
     hipLaunchKernelGGL((conv_backward_kernel<T, W, VEC>), dim3(k.columns * k.rows), dim3(THREADS), 0, stream, make_args<T>(s), g,
                        k.vectors, k.lanes, k.columns, k.slices, k.slice_tokens);
-    const uint32_t columns = (s->channels + 63u) / 64u;
+    const uint32_t columns = sum_columns(s);
     hipLaunchKernelGGL((conv_sum_kernel<W>), dim3(columns * (W + 1)), dim3(64 * SHARES), 0, stream, part, s->channels, columns,
                        k.rows, d_weight, d_bias);
 }
@@ -509,6 +518,7 @@ int ovl_ssm_conv_forward(const ovl_ssm_conv* s, void* y, void* last, void* hip_s
     f.take(y);
     f.take(last);
     const uint32_t vec = f.elements(size);
+    if (const int few = check_lanes("ovl_ssm_conv_forward", s, vec)) return few;
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     switch (s->dtype) {
         case OVL_SSM_FLOAT32: OVL_SSM_BY_WIDTH(forward, float, s, static_cast<float*>(y), static_cast<float*>(last), stream) break;
@@ -520,6 +530,7 @@ int ovl_ssm_conv_forward(const ovl_ssm_conv* s, void* y, void* last, void* hip_s
 
 uint64_t ovl_ssm_conv_workspace_bytes(const ovl_ssm_conv* s) {
     if (check("ovl_ssm_conv_workspace_bytes", s, false) != OVL_SSM_OK) return 0;
+    if (!launchable(sum_columns(s) * (s->width + 1ull), 64 * SHARES)) return 0;
     uint64_t most = 0;                      // whatever access the backward pass will find
     for (uint32_t vec = 16u / size_of(s->dtype); vec >= 1u; vec /= 2u) {
         if (s->channels % vec != 0u) continue;
@@ -545,6 +556,9 @@ int ovl_ssm_conv_backward(const ovl_ssm_conv* s, const ovl_ssm_sequence* d_y, co
     f.take(d_x);
     f.take(d_kept);
     const uint32_t vec = f.elements(size);
+    const cut k = cut_for(s, vec);
+    if (!launchable(sum_columns(s) * (s->width + 1ull), 64 * SHARES) || !launchable((uint64_t)k.columns * k.rows, THREADS))
+        return fail(OVL_SSM_EINVAL, "ovl_ssm_conv_backward: too many elements for one launch");
     if (workspace == nullptr || workspace_bytes < ovl_ssm_conv_workspace_bytes(s) || (reinterpret_cast<uintptr_t>(workspace) & 3u))
         return fail(OVL_SSM_EINVAL, "ovl_ssm_conv_backward: workspace too small or not 4-byte aligned");
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
@@ -567,6 +581,7 @@ int ovl_ssm_conv_step(const ovl_ssm_conv* s, void* y, void* hip_stream) {
     f.take(s->kept, size);
     f.take(y);
     const uint32_t vec = f.elements(size);
+    if (const int few = check_lanes("ovl_ssm_conv_step", s, vec)) return few;
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     switch (s->dtype) {
         case OVL_SSM_FLOAT32: OVL_SSM_BY_WIDTH(step, float, s, static_cast<float*>(y), stream) break;

@@ -1214,6 +1214,7 @@ scan_step_kernel(scan_args<T> p, uint32_t per_sequence, float* state, int64_t st
 
 using ovl_ssm::after_launch;
 using ovl_ssm::fail;
+using ovl_ssm::launchable;
 using ovl_ssm::round_up;
 
 // State entries per lane of a quad: the smallest variant that holds the state.
@@ -1239,6 +1240,13 @@ void chunks_for(plan& p, direction of) {
     p.chunks = p.strands < enough && p.tiles >= 6u ? (uint32_t)(wanted < p.tiles ? wanted : p.tiles) : 1u;
     p.chunk_tiles = (p.tiles + p.chunks - 1u) / p.chunks;
     p.chunks = (p.tiles + p.chunk_tiles - 1u) / p.chunk_tiles;
+}
+
+// Workgroups of the kernel that sums the gradients' parts: for dB and dC, and for the parameters.
+struct sum_grid { uint64_t vector_groups, rest; };
+sum_grid sum_grid_of(const ovl_ssm_scan* s, const plan& p) {
+    const uint64_t vector_all = (uint64_t)s->groups * s->batch * s->length * 2u * s->state;
+    return {(vector_all + 64u * SHARES - 1u) / (64u * SHARES), ((uint64_t)s->channels * (4u * p.entries + 2u) + 63u) / 64u};
 }
 
 // Checks a scan, and plans it.
@@ -1268,12 +1276,16 @@ int check(const char* who, const ovl_ssm_scan* s, direction of, plan& p) {
     p.tiles = (s->length + TILE - 1u) / TILE;
     p.strands = (uint64_t)s->batch * s->groups * p.blocks;
     chunks_for(p, of);
-    // every launch has at most 2^31 - 1 workgroups
-    const uint64_t most = (1ull << 31) - 1;
-    const uint64_t rows = (uint64_t)s->batch * s->channels;
-    if (p.strands * p.chunks > most || rows * 4u * p.entries / THREADS + 1u > most ||
-        (uint64_t)s->batch * s->length > most / 2u * THREADS / ((uint64_t)s->groups * 2u * s->state))
-        return fail(OVL_SSM_EINVAL, name + ": too many elements for one launch");
+    // all launches of the call; the forward pass has four strands to a workgroup, and its join, where the length is split,
+    // few entries
+    bool fits = (uint64_t)s->batch * s->length <= (1ull << 38) / ((uint64_t)s->groups * 2u * s->state);
+    if (of == direction::forward) fits = fits && launchable((p.strands * p.chunks + WAVES - 1) / WAVES, THREADS);
+    if (of == direction::backward) {
+        const sum_grid sums = sum_grid_of(s, p);
+        fits = fits && launchable(p.strands * p.chunks, THREADS) && launchable(sums.vector_groups + sums.rest, 64u * SHARES);
+    }
+    if (token) fits = fits && launchable((uint64_t)s->batch * ((s->channels + BLOCK - 1u) / BLOCK), THREADS);
+    if (!fits) return fail(OVL_SSM_EINVAL, name + ": too many elements for one launch");
     return OVL_SSM_OK;
 }
 
@@ -1381,10 +1393,9 @@ void backward(const ovl_ssm_scan* s, const plan& p, const float* saved, const ov
         hipLaunchKernelGGL((scan_backward_kernel<T, HELD, true, SLICED>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
     else
         hipLaunchKernelGGL((scan_backward_kernel<T, HELD, false, SLICED>), grid, dim3(THREADS), 0, stream, args, to, saved, entry);
-    const uint64_t vector_all = (uint64_t)s->groups * s->batch * s->length * 2u * s->state;
-    const uint32_t vector_groups = (uint32_t)((vector_all + 64u * SHARES - 1u) / (64u * SHARES));
-    const uint32_t rest = (s->channels * (4u * p.entries + 2u) + 63u) / 64u;
-    hipLaunchKernelGGL((scan_gradient_sum_kernel<T>), dim3(vector_groups + rest), dim3(64u * SHARES), 0, stream, to.vector_part,
+    const sum_grid sums = sum_grid_of(s, p);
+    const uint32_t vector_groups = (uint32_t)sums.vector_groups;
+    hipLaunchKernelGGL((scan_gradient_sum_kernel<T>), dim3((uint32_t)(sums.vector_groups + sums.rest)), dim3(64u * SHARES), 0, stream, to.vector_part,
                        to.A_part, to.D_part, to.bias_part, s->batch, s->length, s->channels, s->state, 4u * p.entries,
                        s->groups, p.blocks, s->batch * p.chunks, vector_groups, static_cast<T*>(g->d_B),
                        static_cast<T*>(g->d_C), g->d_A, g->d_D, g->d_delta_bias);

@@ -226,3 +226,46 @@ def test_norms_of_any_number_of_rows_are_taken(libraries):
     for rows in ((1 << 26) + 1, (1 << 31) + 1, (1 << 32) - 1):
         s = rms_norm.Norm(rows, 64, 32, 32, 2, 1e-5, P, 64, None, 0, P)
         assert lib.ovl_norm_workspace_bytes(ctypes.byref(s)) == 2048 * 64 * 4, rows
+
+
+def test_calls_that_one_launch_does_not_take_are_refused(libraries):
+    """A launch has fewer than 2^32 work items; what no kernel of a call could be launched for is refused before any is."""
+    lib, _ = libraries
+    vectors = state_space.Vectors(P, 4, 4, 4)
+    gradients = state_space.ScanGradients(state_space.Sequence(P, 64, 8), None, *([P] * 9))
+
+    def scan(batch, length, channels, state, groups=1):
+        return ctypes.byref(scan_struct(batch=batch, length=length, channels=channels, state=state, groups=groups))
+
+    # the forward pass: a wavefront for 64 channels of a sequence and group
+    taken, much = scan((1 << 26) - 4, 1, 64, 4), scan((1 << 26) - 3, 1, 64, 4)
+    assert lib.ovl_ssm_scan_saved_bytes(taken) > 0 and lib.ovl_ssm_scan_saved_bytes(much) == 0
+    assert lib.ovl_ssm_scan_forward(much, P, P, None, None, 0, None) == EINVAL and b'too many' in lib.ovl_ssm_last_error()
+    # the backward pass: a workgroup of 256; one result of dB and dC per thread; 1024 threads for 64 results of dA, dD, d_bias
+    for taken, much in ((scan((1 << 24) - 1, 1, 64, 4), scan(1 << 24, 1, 64, 4)),
+                        (scan(1, 1 << 24, 64, 64, 1), scan(4, 1 << 23, 64, 64, 1)),
+                        (scan(1, 1, (1 << 22) - (1 << 18), 64), scan(1, 1, 1 << 22, 64))):
+        assert lib.ovl_ssm_scan_workspace_bytes(taken, 1) > 0
+        assert lib.ovl_ssm_scan_workspace_bytes(much, 1) == 0
+        assert lib.ovl_ssm_scan_backward(much, P, ctypes.byref(gradients), P, 1 << 60, None) == EINVAL
+        assert b'too many' in lib.ovl_ssm_last_error()
+    # the step: a workgroup of 256 for 64 channels of a sequence
+    assert lib.ovl_ssm_scan_step(scan(1 << 24, 1, 64, 4), P, 256, P, None) == EINVAL
+    assert b'too many' in lib.ovl_ssm_last_error()
+
+    def conv(batch, channels, odd=0):
+        sequence = state_space.Sequence(P + odd, channels, channels)
+        return ctypes.byref(state_space.Conv(batch, 1, channels, 4, 32, 1, sequence, P, P, sequence, None))
+
+    # the convolution: a thread for the channels of an access
+    for batch, odd in ((1 << 29, 2), ((1 << 32) - 1, 0)):
+        much = conv(batch, 16, odd)
+        assert lib.ovl_ssm_conv_forward(much, P, P, None) == EINVAL and b'too many' in lib.ovl_ssm_last_error()
+        assert lib.ovl_ssm_conv_step(much, P, None) == EINVAL and b'too many' in lib.ovl_ssm_last_error()
+    # its backward pass: at least 8 threads for the accesses of a sequence, and 1024 for 64 channels of a tap's sum
+    d_y = ctypes.byref(state_space.Sequence(P, 64, 64))
+    for much in (conv(1 << 30, 1), conv(2, 1 << 26)):
+        assert lib.ovl_ssm_conv_backward(much, d_y, None, P, P, P, P, P, 1 << 60, None) == EINVAL
+        assert b'too many' in lib.ovl_ssm_last_error()
+    assert lib.ovl_ssm_conv_workspace_bytes(conv(2, 1 << 26)) == 0
+    assert lib.ovl_ssm_conv_workspace_bytes(conv(2, 1 << 25)) > 0
