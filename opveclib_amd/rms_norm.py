@@ -112,8 +112,17 @@ def _rows(t):
     columns = t.shape[-1]
     if t.is_contiguous():
         return t, columns
-    if t.dim() == 2 and (t.stride(1) == 1 or columns == 1):
-        return t, t.stride(0)
+    shape, strides = t.shape, t.stride()
+    if strides[-1] == 1 or columns == 1:
+        distance, rows = None, 1                    # of the rows of the axes seen so far, of which there are that many
+        for size, stride in zip(shape[-2::-1], strides[-2::-1]):
+            if size != 1:
+                if distance is None:
+                    distance = stride
+                elif stride != distance * rows:
+                    return t.contiguous(), columns
+                rows *= size
+        return t, columns if distance is None else distance
     return t.contiguous(), columns
 
 

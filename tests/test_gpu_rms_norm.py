@@ -278,3 +278,30 @@ def test_more_rows_than_one_launch_takes():
         want, want_scales = ref.quantized(rms_norm.rms_norm(s[-4000:].float(), w), group)
         assert torch.equal(scales[-4000:].cpu(), want_scales)
         assert torch.equal(q[-4000:].cpu().view(torch.uint8), want.view(torch.uint8))
+
+
+def test_parts_of_a_projection_are_used_where_they_are():
+    """Halves of [batch, length, 2 columns]: no copies, neither of the rows nor of their gradients."""
+    batch, length, columns = 4, 256, 1000
+    x, r, w, d_y, d_s = inputs(9, (batch, length, 2 * columns), 'bfloat16', 'float32', 'float32')
+    w = w[:columns].contiguous()
+    halves = [t[..., columns:] for t in (x, r, d_y, d_s)]
+    dense = [t.contiguous() for t in halves]
+
+    def work(x, r, d_y, d_s):
+        y, s = rms_norm.rms_norm(x, w, residual=r)
+        return (y, s) + rms_norm.rms_norm_quantized(x, w, residual=r, group=128) + rms_norm.rms_norm_grad(r, w, d_y, d_s, both=True)
+
+    most = []
+    for tensors in (dense, halves):
+        got = work(*tensors)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        again = work(*tensors)
+        most.append(torch.cuda.max_memory_allocated() - before)
+        if tensors is dense:
+            want = got
+    assert most[0] == most[1]
+    for a, b, c in zip(want, got, again):
+        assert torch.equal(a.float(), b.float()) and torch.equal(a.float(), c.float())

@@ -269,3 +269,19 @@ def test_calls_that_one_launch_does_not_take_are_refused(libraries):
         assert b'too many' in lib.ovl_ssm_last_error()
     assert lib.ovl_ssm_conv_workspace_bytes(conv(2, 1 << 26)) == 0
     assert lib.ovl_ssm_conv_workspace_bytes(conv(2, 1 << 25)) > 0
+
+
+def test_rows_at_one_distance_are_not_copied():
+    t = torch.arange(2 * 3 * 4 * 40).view(2, 3, 4, 40).float()
+    for rows, stride in ((t, 40), (t[..., 8:24], 40), (t[:1, ..., :16], 40), (t[:, :, :1, 8:], 160), (t[:, :1, 1, :8], 480),
+                         (t[:, 1:2, :, 3:4], None), (t[0, 0, 0, 1:9], 8), (t[:, 1:2], None), (t[1:, 1:, ::2, 5:], 80),
+                         (t[:1, :1, :1, ::40], 1), (t[0, 0, :, 3:4], 40), (t[..., :16].transpose(1, 2), None),
+                         (t[0, 0, :1].expand(5, 40), 0), (t[0, 0, :1, :8].expand(3, 5, 8), 0), (t[0, 0, 0, ::2], None),
+                         (t[:0, ..., 8:24], 16)):
+        got, got_stride = rms_norm._rows(rows)
+        copied = stride is None
+        assert (got.data_ptr() != rows.data_ptr()) == copied, (rows.shape, rows.stride())
+        columns = rows.shape[-1]
+        assert got_stride == (columns if copied else stride)
+        seen = torch.as_strided(got, (rows.numel() // columns, columns), (got_stride, 1), got.storage_offset())
+        assert torch.equal(seen, rows.reshape(-1, columns))
