@@ -110,6 +110,14 @@ __device__ __forceinline__ float softplus_(float x) {
 
 __device__ __forceinline__ float sigmoid_(float x) { return ovl_lane::rcp_(1.0f + ovl_lane::exp2_(-x * LOG2E)); }
 
+// A in powers of two.  One without bound counts as the largest number: tokens behind the sequence have dt = 0 and change
+// nothing, while 0 times infinity would be NaN.
+__device__ __forceinline__ float rate_(float a) {
+    constexpr float MOST = 0x1.fffffep+127f;
+    const float r = a * LOG2E;
+    return r < -MOST ? -MOST : r > MOST ? MOST : r;
+}
+
 // A sequence tensor as a lane reads it: N tokens of its channel, PACE tokens apart, of a tile of N * PACE tokens.  The
 // tile's address and the tokens' offsets are the same for the whole wavefront and stay in scalar registers; a lane adds 32
 // bits of its own (the host has checked that they suffice).  The offsets are made anew for every tile: kept, those of all
@@ -405,7 +413,7 @@ scan_forward_kernel(scan_args<T> p, uint32_t units, uint32_t chunks, T* y, float
     float h[S], A2[S];
     load_entries(A2, p.A + (uint64_t)w.channel * p.state, 0u, p.state);
 #pragma unroll
-    for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; h[s] = 0.0f; }
+    for (int s = 0; s < S; ++s) { A2[s] = rate_(A2[s]); h[s] = 0.0f; }
     if (entry != nullptr) load_states(h, entry + chunk_row * S, 0u, w.channel, p.channels);
     else if (local == nullptr && p.entering != nullptr) load_entries(h, p.entering + state_row * p.state, 0u, p.state);
     const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
@@ -560,7 +568,7 @@ scan_join_kernel(const float* A, const float* start, float* local, const float* 
     const uint32_t channel = in / 4u % channels, n = in / 4u / channels * 4u + in % 4u;
     const uint64_t row = (uint64_t)b * channels + channel;
     const bool real = n < state;
-    const float A2 = real ? A[(uint64_t)channel * state + n] * LOG2E : 0.0f;
+    const float A2 = real ? rate_(A[(uint64_t)channel * state + n]) : 0.0f;
     float h = real && start != nullptr ? start[row * state + n] : 0.0f;
     for (uint32_t trip = 0; trip < chunks; trip += walkers * AHEAD) {
         const uint32_t base = trip + walker * AHEAD;
@@ -636,7 +644,7 @@ scan_gradient_local_kernel(scan_args<T> p, uint32_t units, sequence<T> d_y, floa
     float r[S], A2[S];
     load_entries(A2, p.A + (uint64_t)w.channel * p.state, 0u, p.state);
 #pragma unroll
-    for (int s = 0; s < S; ++s) { A2[s] *= LOG2E; r[s] = 0.0f; }
+    for (int s = 0; s < S; ++s) { A2[s] = rate_(A2[s]); r[s] = 0.0f; }
     const float bias = p.delta_bias != nullptr ? p.delta_bias[w.channel] : 0.0f;
     const bool gate = p.z.data != nullptr;
     float dt_total = 0.0f;
@@ -788,7 +796,7 @@ scan_backward_kernel(scan_args<T> p, gradient_args<T> g, const float* saved, con
     auto load_A2 = [&](uint32_t slice) {
         load_entries(A2, A_row, slice * 4u + w.q, p.state);
 #pragma unroll
-        for (int s = 0; s < S; ++s) A2[s] *= LOG2E;
+        for (int s = 0; s < S; ++s) A2[s] = rate_(A2[s]);
     };
     for (uint32_t slice = 0; slice < slices; ++slice) {
 #pragma unroll

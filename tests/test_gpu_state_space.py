@@ -679,3 +679,27 @@ def test_states_are_kept_only_where_a_backward_pass_can_follow():
     assert unrecorded == plain and torch.equal(y, y_2) and torch.equal(last, last_2)
     # a state of float32 per channel and 16 tokens
     assert recorded >= plain + 4 * 1024 * 512 * 16 * 4 // 16
+
+
+@pytest.mark.parametrize('length', [3, 64, 333])
+def test_entries_that_forget_at_once(length):
+    """A without bound, or beyond float32 with a factor: the decay is zero for every token, and tokens behind the sequence
+    change nothing.  The gradients are those of decays that are zero in all bits, as for A = -1e6."""
+    d = ref.scan_inputs(78, 3, length, 4, 9, 2, 'float32', ragged=True, device='cuda')
+    d['A'][0, 0] = d['A'][3, 8] = -1e6
+    cpu = {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+    want_y, want_last, want = ref.scan_expected(cpu)
+    d['A'][0, 0], d['A'][3, 8] = float('-inf'), -3.2e38
+    y, last = run_scan(d)
+    close(y, want_y, F32, 'y', 16)
+    close(last, want_last, F32, 'last', 16)
+    for name, got, w in zip(ref.SCAN_NAMES, run_grad(d), want):
+        close(got, w, F32, 'd_' + name, 64)
+    state = d['state'].clone()
+    token = {k: d[k][:, 0].contiguous() for k in ('u', 'delta', 'z', 'B', 'C')}
+    y = state_space.scan_step(state, token['u'], token['delta'], d['A'], token['B'], token['C'], D=d['D'], z=token['z'],
+                              delta_bias=d['delta_bias'], softplus=True)
+    first = {k: (v[:, :1] if k in token else v) for k, v in cpu.items()}
+    want_y, want_last, _ = ref.scan_expected(dict(first, lengths=None, d_y=cpu['d_y'][:, :1]))
+    close(y, want_y[:, 0], F32, 'y of the step', 16)
+    close(state, want_last, F32, 'state of the step', 16)

@@ -132,6 +132,45 @@ def test_scan_backward(program, case):
             close(g, w, kind if name in ('u', 'delta', 'z', 'B', 'C') else f32, 'd_' + name, 32)
 
 
+def forget_at_once(A):
+    """Some decays exp(dt A) that are zero whatever the time step: A without bound, or beyond float32 with a factor."""
+    A[0, 0], A[-1, -1] = float('-inf'), -3.2e38
+    return A
+
+
+@pytest.mark.parametrize('case', [(1, 13, 3, 5, 1, 'float32', True, False, True, True),
+                                  (3, 24, 2, 16, 1, 'float32', False, True, True, False),
+                                  (2, 230, 2, 8, 1, 'bfloat16', False, True, True, True)], ids=str)
+def test_scan_forward_with_entries_that_forget_at_once(program, case):
+    """Tokens behind the sequence change no state, also where nothing decays for them and everything for others."""
+    batch, length, channels, n, groups, dtype = case[:6]
+    d = scan_case(case, 9)
+    forget_at_once(d['A'])
+    ins = [d['u'], d['delta'], d['z'], d['B'], d['C'], d['A'], d['D'], d['delta_bias'], d['state'], d['lengths']]
+    kind = ref.TYPES[dtype]
+    y, last, _ = run(program, scan_settings(case, 0, 0), ins,
+                     [((batch, length, channels), kind), ((batch, channels, n), torch.float32), ((0,), torch.float32)])
+    want_y, want_last, _ = ref.scan_expected(d)
+    close(y, want_y, kind, 'y', 16)
+    close(last, want_last, torch.float32, 'last', 16)
+
+
+def test_scan_backward_with_entries_that_forget_at_once(program):
+    """Their gradients are those of decays that are zero in all bits (for A = -1e6: every time step is 1e-4 and more)."""
+    case = (2, 21, 3, 5, 1, 'float32', True, True, True, True)
+    batch, length, channels, n, groups, dtype = case[:6]
+    d = scan_case(case, 10)
+    _, _, want = ref.scan_expected(dict(d, A=torch.where(forget_at_once(d['A'].clone()) > -1e30, d['A'], -1e6)))
+    forget_at_once(d['A'])
+    ins = [d['u'], d['delta'], d['z'], d['B'], d['C'], d['A'], d['D'], d['delta_bias'], d['state'], d['lengths'], d['d_y'], d['d_last']]
+    f32 = torch.float32
+    outs = [((batch, length, channels), f32), ((batch, length, channels), f32), ((channels, n), f32), ((batch, length, groups, n), f32),
+            ((batch, length, groups, n), f32), ((channels,), f32), ((batch, length, channels), f32), ((channels,), f32),
+            ((batch, channels, n), f32)]
+    for name, g, w in zip(ref.SCAN_NAMES, run(program, scan_settings(case, 1, 0), ins, outs), want):
+        close(g, w, f32, 'd_' + name, 32)
+
+
 @pytest.mark.parametrize('case', [(1, 1, 1, 1, 1, 'float32', False, False, True, True),
                                   (3, 1, 70, 16, 2, 'bfloat16', True, False, True, True),
                                   (2, 1, 21, 30, 3, 'float16', True, False, True, False),
