@@ -703,3 +703,28 @@ def test_entries_that_forget_at_once(length):
     want_y, want_last, _ = ref.scan_expected(dict(first, lengths=None, d_y=cpu['d_y'][:, :1]))
     close(y, want_y[:, 0], F32, 'y of the step', 16)
     close(state, want_last, F32, 'state of the step', 16)
+
+
+def test_scans_whose_outputs_have_more_than_32_bits_of_bytes():
+    """One sequence many times over: every one of the results is the first's."""
+    batch, length, channels, n = 1040, 505, 4096, 3
+    one = ref.scan_inputs(79, 1, length, channels, n, 1, 'bfloat16', device='cuda')
+    every = {k: v.expand((batch,) + v.shape[1:]) if k in ('u', 'delta', 'z', 'B', 'C', 'state', 'd_y', 'd_last') else v
+             for k, v in one.items()}
+    assert batch * length * channels > 2 ** 31
+    y, last = run_scan(every)
+    want_y, want_last, want = ref.scan_expected({k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in one.items()})
+    # A token's decay is off by a unit in its last place (2^-23) and its fused multiply-add by half of one: 0.75 times 2^-22 of
+    # a state that forgets little in 505 tokens, at random sqrt(505) * 0.75 = 17 together, and 4.5 times that, 76, for the
+    # largest of the 12288 states; the gradient that passes through the sequence likewise.
+    terms = 80
+    close(y[:1], want_y, torch.bfloat16, 'y', terms)
+    close(last[:1], want_last, F32, 'last', terms)
+    for part in y.split(130) + last.split(130):
+        assert torch.equal(part, (y if part.dtype == y.dtype else last)[:1].expand_as(part))
+    del y, last
+    for name, got, w in zip(ref.SCAN_NAMES, run_grad(every), want):
+        if got.shape[0] == batch:
+            close(got[:1], w, got.dtype, 'd_' + name, terms)
+            for part in got.split(130):
+                assert torch.equal(part, got[:1].expand_as(part)), name
