@@ -10,9 +10,9 @@
 // (4096 rows of 20000 columns in bf16 with the residual: 155 us with the second, else 149).  Rows need not start on vector boundaries: the vectors are
 // accessed with the alignment of an element, a row's last, partial vector element by element.
 //
-// Measured: 16384 rows of 8192 columns in bf16 with the residual's addition, to 8 bits with a scale per 128 columns, 173 us
+// Measured: 16384 rows of 8192 columns in bf16 with the residual's addition, to 8 bits with a scale per 128 columns, 175 us
 // (939 MB, 5.4 TB/s, what a large copy reaches); 8192 rows of 4096 in bf16 with float32 sums, forward 74 us (5.4 TB/s),
-// backward 104 us (5.2 TB/s) and 4 us for the weights' sums; 5 rows of 4096 to 8 bits 3.7 us (latency).
+// backward 105 us (5.1 TB/s) and 5 us for the weights' sums; 5 rows of 4096 to 8 bits 4.0 us (latency).
 #include <math.h>
 #include <stdint.h>
 #include <string>
@@ -261,7 +261,8 @@ norm_backward_kernel(norm_args p, norm_gradient_args g, uint32_t teams) {
     // a row's inputs are read one row ahead where there are registers for it (8192 rows of 4096 columns, bf16 with float32
     // sums: 106 us, else 113).  A team of 1024 lanes has 128 registers for each and does not read ahead (4096 rows of 16384:
     // 208 us, 342 with rows ahead in scratch memory); with four vectors per lane it reads a row twice, the second time from
-    // the L2, and holds nothing of it in between (2048 rows of 32768: 284 us, 424 held in scratch memory).
+    // the L2, and holds no inputs in between (2048 rows of 32768: 284 us, 3.8 TB/s, 424 with them in scratch memory; 9 to 13
+    // registers of each lane still go there).
     constexpr bool AHEAD = HELD <= 2 && LANES <= 256, LEAN = HELD > 2 && LANES > 256;
     float w[HELD][VEC];
     if (!LEAN)

@@ -8,8 +8,8 @@
 // Work layout: a lane owns VEC neighbouring channels (16 bytes where sizes and addresses allow it) and walks along tokens
 // with the last inputs in registers, so every input is loaded once but for the few tokens before a walk's first.  All of
 // it is bound by memory: the forward pass reads x and writes y, the backward pass reads x and dy and writes dx.  Measured
-// on 4 sequences of 4096 tokens, 8192 channels, width 4, bf16 (x a half of a projection): forward 97 us, 5.5 TB/s, as much
-// as a large copy reaches; backward 180 to 200 us, 4.0 to 4.5 TB/s; one token of 64 sequences of 4096 channels 3.8 us.
+// on 4 sequences of 4096 tokens, 8192 channels, width 4, bf16 (x a half of a projection): forward 97 to 102 us, 5.3 to 5.5
+// TB/s, as much as a large copy reaches; backward 176 to 210 us, 3.9 to 4.6 TB/s; one token of 64 sequences of 4096 channels 3.8 us.
 #include <math.h>
 
 #include "ovl_lane.h"

@@ -19,7 +19,7 @@
 // and a chunk, nothing is summed across lanes, and there is no barrier.  B and C, the same for the whole wavefront, come
 // from the lanes of a row as operands of the consuming instructions and through a part of LDS of its own.  Addresses are
 // scalar with 32 bits per lane.  (With a quad per channel the forward pass of 4 sequences of 2048 tokens, 4096 channels of
-// 16 entries in bf16 took 373 us without a split, now it takes 270 with both passes.)
+// 16 entries in bf16 took 373 us without a split, now it takes 248 with both passes and the join.)
 // The backward pass holds states and decays of several tokens, and sums over channels: a quad owns a channel and its
 // lanes a quarter of the state each; what depends on (token, channel) only is done once for four tokens in the four lanes
 // and handed round with lane moves; sums over the state end in an exchange that leaves every lane with its own token.
@@ -390,9 +390,9 @@ template <int S, uint32_t TOKENS, bool BACKWARD> struct vector_queue {
 // S entries (all of a state, padded) in the lane of their channel: nothing has to be summed across lanes.  A wavefront owns
 // 64 channels and a chunk and takes STEP tokens at a time, the next ones' loads in flight.  The four wavefronts of a
 // workgroup have nothing to do with each other; they are one workgroup so that every SIMD of a compute unit gets one.
-// 4 sequences of 2048 tokens, 4096 channels of 16 entries, bf16: full pass with kept states 151 us, pass over states only
-// 105 us, where the recurrence's instructions alone take 82 (with the output) and 64 us; the rest is softplus, the gate,
-// conversions and addresses, once per token and channel.  One sequence of 8192 tokens, 2048 channels: 76 and 56 us.
+// 4 sequences of 2048 tokens, 4096 channels of 16 entries, bf16: full pass with kept states 143 us, pass over states only
+// 97 us, where the recurrence's instructions alone take 82 (with the output) and 64 us; the rest is softplus, the gate,
+// conversions and addresses, once per token and channel.  One sequence of 8192 tokens, 2048 channels: 71 and 51 us.
 // OUTPUT: the full pass (y, the last state, the kept states).  Otherwise only states: the chunk's own effect on a zero
 // state (`local`, `dt_sum`), or the kept states.
 template <typename T, int S, bool OUTPUT>
@@ -548,7 +548,7 @@ scan_forward_kernel(scan_args<T> p, uint32_t units, uint32_t chunks, T* y, float
 // (sequence, channel, state entry) in a row, which it reads before any is overwritten, and `walkers` threads (a power of
 // two) stand behind one another: each makes one step (decay, effect) of its chunks, the states between them are joined
 // through LDS, and each hands its own state on.  So 128 chunks are one trip of 16 walkers, where a thread alone would wait
-// for memory 16 times (128 chunks of 2048 channels of 16 entries: 19.6 us alone, 9.5 with 16 walkers).  REVERSE: the gradient's recurrence, which
+// for memory 16 times (128 chunks of 2048 channels of 16 entries: 19.6 us alone, 9.2 with 16 walkers).  REVERSE: the gradient's recurrence, which
 // enters chunks from their ends.
 constexpr uint32_t AHEAD = 8, MOST_WALKERS = 16;
 constexpr uint32_t join_ids(uint32_t walkers) { return walkers < 4u ? THREADS / walkers : 64u; }
@@ -767,7 +767,7 @@ template <int S> struct channel_sums {
 // as float32, one barrier per tile for them and one for the sums.
 //
 // Bound by the vector ALU: 26 instructions per token and 64 entries (14 of the recurrences, 4.5 of the sums over channels,
-// 2 of the states computed twice, the rest per token and channel), and the vector ALU is busy for 380 of the 490 to 530 us
+// 2 of the states computed twice, the rest per token and channel), and the vector ALU is busy for 380 of the 465 us
 // that 4 sequences of 2048 tokens, 4096 channels of 16 entries in bf16 take.
 //
 // SLICED: states of more than 16 entries are taken 16 at a time, tile by tile, and what a lane keeps of the other slices is
@@ -1144,7 +1144,8 @@ scan_gradient_sum_kernel(const float* vector_part, const float* A_part, const fl
 // ---------------------------------------------------------------------------------------------------------------------
 
 // The recurrence once: a quad per (sequence, channel), a workgroup for 64 channels of a sequence.  Bound by reading and
-// writing the state: 96 sequences of 4096 channels, 16 entries, bf16: 54 MB in 11.0 us, 4.9 TB/s; 2 of 1024: 3.0 us.
+// writing the state: 96 sequences of 4096 channels, 16 entries, bf16: 54 MB in 12.6 us, 4.3 TB/s (the same
+// states again at once, which are still in the caches: 11.0 us); 2 of 1024: 3.0 us.
 // WHOLE: a lane's S entries are all there, and accessed as vectors of 16 (S = 2: 8) aligned bytes.
 template <typename T, int S, bool WHOLE>
 __global__ void __launch_bounds__(THREADS)
@@ -1235,8 +1236,10 @@ struct plan {
 
 enum class direction { forward, backward, token };
 
-// Into how many chunks the length is split: into so many that every SIMD has four wavefronts of the passes with a channel
-// per lane, where the split pays for its second evaluation of the decays.  4096 channels of 16 entries, bf16:
+// Into how many chunks the length is split, where the split pays for its second evaluation of the decays: into so many that
+// the passes with a channel per lane have 4096 wavefronts, four for each SIMD.  Not all of them are resident together in every
+// variant: with 8, 16, 32, 64 entries the full pass has registers for 4, 3, 2, 1 wavefronts on a SIMD, the forward pass over
+// states for 6, 4, 3, 1, the gradient's for 5, 4, 3, 2; the others start as these end.  4096 channels of 16 entries, bf16:
 //   forward    below 1024 strands (one wavefront per SIMD without a split): 12 sequences of 2048 tokens, 768 strands, take
 //              694 us split and 761 else, 16 sequences 813 split and 768 else
 //   backward   below 512, since a strand is four wavefronts of its main kernel: 4 sequences, 256 strands, take 598 us split
