@@ -198,14 +198,14 @@ norm_forward_kernel(norm_args p, T* y, R* summed, uint8_t* q, float* scales) {
         }
     // The smallest scale is the smallest normal number: the last bits of one below would not be there.  y is divided by it: a
     // product with a rounded reciprocal would move values in the middle of two e4m3 numbers, so the reciprocal is carried to
-    // twice the precision, which makes the product the rounded quotient, but for the last bit of one in a million (where the
-    // low part is a normal number, for scales up to 2^100).  Its first part is too small by more than its error, so that the second is positive and zeros keep
-    // their sign.
+    // twice the precision, which makes the product the rounded quotient, but for the last bit of one in a million.  Its first
+    // part is too small by more than its error, so that the second is positive and zeros keep their sign; the second is
+    // subnormal for the largest scales, where the eight bits that it has left suffice.
     float scale, high, low;
     auto scale_by = [&](float top) {
         scale = top > 0.0f ? fmaxf(top / E4M3_MAX, 0x1p-126f) : 1.0f;
         high = ovl_lane::rcp_(scale) * (1.0f - 0x1p-22f);
-        low = scale <= 0x1p100f ? fmaf(-high, scale, 1.0f) * high : 0.0f;
+        low = scale <= 0x1.fffffep+127f ? fmaf(-high, scale, 1.0f) * high : 0.0f;
     };
     if (!GROUPED) {
         scale_by(across<LANES, max_op>(row_top, lds[1]));

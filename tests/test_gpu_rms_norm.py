@@ -305,3 +305,15 @@ def test_parts_of_a_projection_are_used_where_they_are():
     assert most[0] == most[1]
     for a, b, c in zip(want, got, again):
         assert torch.equal(a.float(), b.float()) and torch.equal(a.float(), c.float())
+
+
+@pytest.mark.parametrize('power', [-115, 108])
+def test_middles_of_very_small_and_large_results_go_to_the_even_one(power):
+    weights, t = ref.middles(list(range(1, 200, 2)) + [509, 511])
+    want = t.float().to(torch.float8_e4m3fn).view(torch.uint8).cuda()
+    ones = torch.ones(2, 128, device='cuda')
+    for row in weights * 2.0 ** power:
+        for group in (None, 128):
+            q, scales = rms_norm.rms_norm_quantized(ones, row.cuda(), eps=0.0, group=group)
+            assert bool((scales == row[0].item() / 448).all())
+            assert torch.equal(q.view(torch.uint8), want.expand(2, 128))

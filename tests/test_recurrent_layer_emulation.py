@@ -364,3 +364,15 @@ def test_norm_in_several_launches(program, rows, columns):
         exact = want / want_scales.repeat_interleave(group or columns, 1)[:, :columns]
         # one rounding to four significant bits (2^-10 in the subnormal range), and float32 arithmetic before it
         assert bool(((q.double() - exact).abs() <= exact.abs() * (2.0 ** -4 + 2.0 ** -20) + 2.0 ** -10).all())
+
+
+@pytest.mark.parametrize('power', [-115, 108])
+def test_norm_to_8_bits_sends_middles_of_very_small_and_large_results_to_the_even_number(program, power):
+    weights, t = ref.middles([1, 3, 7, 49, 511])
+    ones = torch.ones(1, 128)
+    for row in weights * 2.0 ** power:
+        for group in (0, 128):
+            q, scales, _ = run(program, [7, 1, 128, 2, 2, 2, 128, 128, group, 1], [ones, None, row],
+                               [((1, 128), torch.float8_e4m3fn), ((1, 1), torch.float32), ((0,), torch.float32)])
+            assert scales.item() == row[0].item() / 448
+            assert torch.equal(q.view(torch.uint8)[0], t.float().to(torch.float8_e4m3fn).view(torch.uint8))
