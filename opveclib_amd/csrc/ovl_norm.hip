@@ -7,8 +7,8 @@
 // Work layout: LANES lanes share a row (a wavefront, four or sixteen of them) and hold all of it in registers, HELD
 // vectors of eight columns per lane, so everything is read once and written once: the kernels are bound by memory.  The
 // statistics of a row are one exchange between its wavefronts, the largest result for a scale that spans the row another
-// (4096 rows of 20000 columns in bf16 with the residual: 155 us with the second, else 149).  Rows need not start on vector boundaries: the vectors are
-// accessed with the alignment of an element, a row's last, partial vector element by element.
+// (4096 rows of 20000 columns in bf16 with the residual: 155 us with the second, else 149).  Rows need not start on vector
+// boundaries: the vectors are accessed with the alignment of an element, a row's last, partial vector element by element.
 //
 // Measured: 16384 rows of 8192 columns in bf16 with the residual's addition, to 8 bits with a scale per 128 columns, 175 us
 // (939 MB, 5.4 TB/s, what a large copy reaches); 8192 rows of 4096 in bf16 with float32 sums, forward 74 us (5.4 TB/s),
